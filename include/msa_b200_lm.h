@@ -138,6 +138,23 @@ typedef struct {
 } msa_lm_group_args;
 int msa_lm_group_prep(const msa_lm_group_args* args, void* stream);
 
+/* ---- windows with first tokens that stay visible ----------------------------------------------------------------------
+ * The functions without `first` are those of first = 0.  With it, position i sees j <= i with i - j < window or j < first.  A ring
+ * (of first + window rows at least) keeps position p in row p while p < first, and in row first + (p - first) % (ring_rows - first)
+ * from there on.  The context of a portion begins with the min(start, first + window - 1) earlier positions that its first
+ * token sees: the first tokens, then the window; its own rows follow. */
+int msa_lm_group_prep_first(const msa_lm_group_args* args, int32_t first, void* stream);
+int msa_lm_ring_store_first(const void* ctx, int32_t row_width, const int32_t* slot, const int32_t* start, const int32_t* cu,
+                            const int32_t* ctx_off, int32_t n_seq, int32_t n_decode, int32_t max_len, int32_t window, int32_t first,
+                            void* ring, int64_t ring_rows, int32_t dtype, void* stream);
+int msa_lm_window_attn_first(const msa_lm_attn_args* args, int32_t first, void* stream);
+int msa_lm_window_attn_tc_first(const msa_lm_attn_args* args, int32_t first, int32_t n_rows, int32_t n_ctx, int32_t row0, int32_t* status,
+                                void* stream);
+int msa_lm_group_decode_first(const void* q, int64_t q_row, const void* ring, int64_t ring_rows, const int32_t* slot, const int32_t* pos,
+                              int32_t n, int32_t heads, int32_t kv_heads, int32_t dim, int32_t vdim, int32_t window, int32_t first,
+                              int32_t splits, float scale, int32_t sink, const void* gate, int64_t gate_row, void* out, int64_t out_row,
+                              float* part_o, float* part_ml, void* stream);
+
 /* Convolution inputs of the last taps-1 positions of every non-decode sequence -> conv_state; `proj` points at the first
  * convolved column of the packed rows. */
 int msa_lm_conv_store(const void* proj, int64_t proj_stride, int32_t channels, int32_t taps, void* conv_state, const int32_t* slot,

@@ -18,7 +18,8 @@ EXPORTS = ["msa_lm_residual_norm", "msa_lm_embed", "msa_lm_silu_mul", "msa_lm_so
            "msa_lm_ssd_chunk_supported", "msa_lm_ssd_chunk", "msa_lm_ssd_walk_supported", "msa_lm_ssd_walk", "msa_lm_part_norm", "msa_lm_latent_prep", "msa_lm_ring_store",
            "msa_lm_window_attn", "msa_lm_window_attn_tc_supported", "msa_lm_window_attn_tc", "msa_lm_latent_decode_supported", "msa_lm_latent_decode", "msa_lm_delta_decode", "msa_lm_delta_prep", "msa_lm_delta_prep_split", "msa_lm_delta_chunk_supported", "msa_lm_delta_chunk_workspace", "msa_lm_delta_chunk", "msa_lm_gather_rows", "msa_lm_delta_conv_store", "msa_lm_delta_scan",
            "msa_lm_delta_out", "msa_lm_moe_topk", "msa_lm_moe_sort", "msa_lm_moe_gemm", "msa_lm_moe_gemm_tc",
-           "msa_lm_rows_gemm", "msa_lm_argmax"]
+           "msa_lm_rows_gemm", "msa_lm_argmax", "msa_lm_group_prep_first", "msa_lm_ring_store_first", "msa_lm_window_attn_first",
+           "msa_lm_window_attn_tc_first", "msa_lm_group_decode_first"]
 
 vp, i32, i64, f32 = C.c_void_p, C.c_int32, C.c_int64, C.c_float
 
@@ -122,6 +123,11 @@ def lib() -> C.CDLL:
             "msa_lm_window_attn": [ap, vp],
             "msa_lm_window_attn_tc_supported": [i32, i32, i32],
             "msa_lm_window_attn_tc": [ap, i32, i32, i32, vp, vp],
+            "msa_lm_group_prep_first": [C.POINTER(GroupArgs), i32, vp],
+            "msa_lm_ring_store_first": [vp, i32, vp, vp, vp, vp, i32, i32, i32, i32, i32, vp, i64, i32, vp],
+            "msa_lm_window_attn_first": [ap, i32, vp],
+            "msa_lm_window_attn_tc_first": [ap, i32, i32, i32, i32, vp, vp],
+            "msa_lm_group_decode_first": [vp, i64, vp, i64, vp, vp, i32, i32, i32, i32, i32, i32, i32, i32, f32, i32, vp, i64, vp, i64, vp, vp, vp],
             "msa_lm_latent_decode_supported": [i32, i32],
             "msa_lm_latent_decode": [vp, i64, i64, vp, i64, i64, vp, i64, vp, vp, i32, i32, i32, i32, i32, i32, f32, vp, vp, vp, vp, vp],
             "msa_lm_moe_gemm_tc": [vp, i64, i32, vp, vp, i32, vp, vp, i32, i32, i32, i32, f32, vp, i64, vp, vp],

@@ -70,11 +70,27 @@ class SparseCacheOnCPU(SparseCache):
 @dataclass(frozen=True)
 class RingSpec:
     """A windowed layer's state: the last rows of ``width`` elements (``window`` None: every row) and, where a short
-    convolution feeds them, its last ``taps - 1`` inputs over ``channels`` channels."""
+    convolution feeds them, its last ``taps - 1`` inputs over ``channels`` channels.  ``first``: rows of the first tokens, which
+    stay; they come in front of the ``window`` others."""
     width: int
     window: Optional[int]
     channels: int = 0
     taps: int = 1
+    first: int = 0
+
+    def __post_init__(self):
+        if self.first < 0 or (self.window is not None and self.window < 1):
+            raise ValueError(f"RingSpec: window {self.window} with {self.first} first tokens")
+
+    def rows(self, max_len: int) -> int:
+        return max_len if self.window is None else min(self.window + self.first, max_len)
+
+
+def window_of(key, max_len: int) -> Tuple[int, int]:
+    """``(window, first)`` of an attention window in a cache of ``max_len`` positions.  ``key``: tokens that a query sees, itself
+    included (None: all), or ``(tokens, first tokens that stay visible beside them)``.  A cache that holds no more than they see has one window."""
+    window, first = key if isinstance(key, tuple) else (key, 0)
+    return (max_len, 0) if window is None or window + first >= max_len else (window, first)
 
 
 @dataclass(frozen=True)
@@ -96,7 +112,7 @@ class SequenceStateCache(SparseCache):
     One slot holds a sequence's state in every layer run; ``acquire`` / ``release`` hand slots out and take them back.
     Nothing is cleared: the kernels take a sequence at position 0 as empty and never read a ring row that the sequence
     has not written.  One more slot than asked for exists, ``scratch``: rows that only fill up a step work there.  ``specs`` lists the runs in order (``model.state_specs()``); a ring has
-    ``min(window, max_len)`` rows.  ``last_token`` keeps every sequence's previous token (for embeddings that read it).  The protocol of ``SparseCache`` (``meta``, ``record_kwargs``) stays usable, so the
+    ``min(window + first, max_len)`` rows.  ``last_token`` keeps every sequence's previous token (for embeddings that read it).  The protocol of ``SparseCache`` (``meta``, ``record_kwargs``) stays usable, so the
     interleave loop drives a model on this cache unchanged."""
 
     def __init__(self, specs: Sequence, n_slots: int, max_len: int, device, dtype: torch.dtype):
@@ -112,8 +128,7 @@ class SequenceStateCache(SparseCache):
         self.last_token = torch.zeros(rows_all, dtype=torch.int32, device=device)
         for i, s in enumerate(self.specs):
             if isinstance(s, RingSpec):
-                rows = max_len if s.window is None else min(s.window, max_len)
-                self.ring[i] = torch.zeros((rows_all, rows, s.width), dtype=dtype, device=device)
+                self.ring[i] = torch.zeros((rows_all, s.rows(max_len), s.width), dtype=dtype, device=device)
             else:
                 self.state[i] = torch.zeros((rows_all, s.heads, s.dim, s.vdim), dtype=torch.float32, device=device)
                 if s.shift:
@@ -159,12 +174,13 @@ class SequenceStateCache(SparseCache):
 @dataclass
 class ContextView:
     """Context bookkeeping of one step for one attention window: where each portion's context starts (``ctx_off``,
-    prefix sums) and how many earlier rows it begins with (``old_off``, prefix sums)."""
+    prefix sums) and how many earlier rows it begins with (``old_off``, prefix sums).  ``first``: tokens that stay visible."""
     window: int
     ctx_off: Optional[torch.Tensor]
     old_off: Optional[torch.Tensor]
     n_ctx: int
     n_old: int
+    first: int = 0
 
 
 class PackedStep:
@@ -203,13 +219,13 @@ class PackedStep:
         want = [row0[i] + w for i, (_, _, ws) in enumerate(entries) for w in ws]
         views = []
         for window in windows:
-            size = cache.max_len if window is None else min(window, cache.max_len)
+            size, first = window_of(window, cache.max_len)
             ctx, old = [0], [0]
             for k in range(self.n_decode, self.n_seq):
-                o = min(start[k], size - 1)
+                o = min(start[k], first + size - 1)
                 old.append(old[-1] + o)
                 ctx.append(ctx[-1] + o + cu[k + 1] - cu[k])
-            views.append((window, size, ctx, old))
+            views.append((window, (size, first), ctx, old))
         chunk_off = [0]                       # chunks of 64 tokens of the portions (the recurrent layers walk those)
         for k in range(self.n_decode, self.n_seq):
             chunk_off.append(chunk_off[-1] + (cu[k + 1] - cu[k] + 63) // 64)
@@ -225,8 +241,8 @@ class PackedStep:
             dev.append(flat[at:at + len(p)])
             at += len(p)
         self.token, self.pos, self.tok_seq, self.slot, self.start, self.cu, self.want_rows, self.chunk_off = dev[:8]
-        self.views = {w: ContextView(size, dev[8 + 2 * i], dev[9 + 2 * i], ctx[-1], old[-1])
-                      for i, (w, size, ctx, old) in enumerate(views)}
+        self.views = {w: ContextView(size, dev[8 + 2 * i], dev[9 + 2 * i], ctx[-1], old[-1], first)
+                      for i, (w, (size, first), ctx, old) in enumerate(views)}
 
     def commit(self, cache: SequenceStateCache) -> None:
         """The step has been launched: its sequences have grown."""
@@ -250,7 +266,10 @@ class DecodeStep:
         self.tok_seq = torch.arange(n, **i)
         self.cu = torch.arange(n + 1, **i)
         self.want_rows = torch.arange(n, **i)
-        self.views = {w: ContextView(cache.max_len if w is None else min(w, cache.max_len), None, None, 0, 0) for w in windows}
+        self.views = {}
+        for w in windows:
+            size, first = window_of(w, cache.max_len)
+            self.views[w] = ContextView(size, None, None, 0, 0, first)
         self._host = torch.zeros((3, n), dtype=torch.int32)
         self._copied = None
         if dev.type == "cuda":

@@ -89,6 +89,19 @@ __device__ __forceinline__ int owner_of(const int32_t* off, int n, int i) {
   return lo;
 }
 
+// Windows with first tokens that stay visible: position i sees j <= i with i - j < window or j < first.  A ring keeps the first
+// positions in its first rows and walks the others through the rest, at least `window` rows.
+__device__ __forceinline__ int ring_row(int pos, int first, int rows) { return pos < first ? pos : first + (pos - first) % (rows - first); }
+// The context of a portion that starts at `start` begins with the earlier positions that its first token sees (its query sees itself
+// and span - 1 others, span = first + window): the first ones and the last ones, or all of them while they are that few.
+__device__ __forceinline__ int old_rows(int start, int span) { return min(start, span - 1); }
+__device__ __forceinline__ int old_position(int k, int start, int first, int span) { return k < first ? k : start - old_rows(start, span) + k; }
+inline int ring_size(int64_t rows) { return rows < 0x7fffffff ? (int)rows : 0x7fffffff; }   // positions are below that
+// What a launcher asks of a window with first tokens: rows for both, and spans that fit 32 bits.
+inline bool first_fits(int first, int window, int64_t ring_rows) {
+  return first == 0 || (first > 0 && window > 0 && first <= 0x7fffffff - window && (ring_rows == 0 || ring_rows >= (int64_t)first + window));
+}
+
 #define MSA_LM_DISPATCH(dtype, ...)                                   \
   do {                                                                \
     if ((dtype) == MSA_BF16) { using T = __nv_bfloat16; __VA_ARGS__ } \

@@ -1,8 +1,8 @@
 // Grouped-query attention behind a short convolution: what happens between the projections and the attention proper
 // (convolution, rotation, ring and context upkeep), and decode attention over the ring.
 //
-// Per sequence slot a layer keeps a ring of the last `ring_rows` rows [keys | values] (position p in row p % ring_rows) and
-// the last taps-1 inputs of the convolutions.  A step that brings several tokens of a sequence works on a packed context:
+// Per sequence slot a layer keeps a ring of the last `ring_rows` rows [keys | values] (position p in row p % ring_rows; with first
+// tokens that stay visible these have rows of their own in front) and the last taps-1 inputs of the convolutions.  A step that brings several tokens of a sequence works on a packed context:
 // the ring rows its first token still sees, then its own rows; the ring takes over the last of them afterwards.
 #include "lm_conv.cuh"
 #include "lm_merge.cuh"
@@ -38,17 +38,17 @@ __device__ __forceinline__ GroupColumn group_column(const msa_lm_group_args& a, 
   return g;
 }
 template <typename T>
-__device__ __forceinline__ T* group_row(const msa_lm_group_args& a, const GroupLayout& L, long long n, int s, int t, int p0) {
-  if (n < a.n_decode) return reinterpret_cast<T*>(a.ring) + ((long long)a.slot[s] * a.ring_rows + p0 % a.ring_rows) * L.width;
-  return reinterpret_cast<T*>(a.ctx) + (long long)(a.ctx_off[s - a.n_decode] + min(p0, a.window - 1) + t) * L.width;
+__device__ __forceinline__ T* group_row(const msa_lm_group_args& a, const GroupLayout& L, int first, int rows, long long n, int s, int t, int p0) {
+  if (n < a.n_decode) return reinterpret_cast<T*>(a.ring) + ((long long)a.slot[s] * a.ring_rows + ring_row(p0, first, rows)) * L.width;
+  return reinterpret_cast<T*>(a.ctx) + (long long)(a.ctx_off[s - a.n_decode] + old_rows(p0, first + a.window) + t) * L.width;
 }
 
 // An old ring row that a continued portion still sees goes to the context.
 template <typename T, int V>
-__device__ __forceinline__ void copy_old_row(const msa_lm_group_args& a, const GroupLayout& L, int o) {
+__device__ __forceinline__ void copy_old_row(const msa_lm_group_args& a, const GroupLayout& L, int first, int rows, int o) {
   const int ps = owner_of(a.old_off, a.n_seq - a.n_decode, o), s = ps + a.n_decode;
-  const int k = o - a.old_off[ps], start = a.start[s], first = start - min(start, a.window - 1);
-  const T* src = reinterpret_cast<const T*>(a.ring) + ((long long)a.slot[s] * a.ring_rows + (first + k) % a.ring_rows) * L.width;
+  const int k = o - a.old_off[ps], pos = old_position(k, a.start[s], first, first + a.window);
+  const T* src = reinterpret_cast<const T*>(a.ring) + ((long long)a.slot[s] * a.ring_rows + ring_row(pos, first, rows)) * L.width;
   T* dst = reinterpret_cast<T*>(a.ctx) + (long long)(a.ctx_off[ps] + k) * L.width;
   for (int i = threadIdx.x * V; i < L.width; i += blockDim.x * V) {
     if constexpr (V == 4) store4(dst + i, load4(src + i));
@@ -58,10 +58,10 @@ __device__ __forceinline__ void copy_old_row(const msa_lm_group_args& a, const G
 
 // Any sizes: a block per packed row; a rotated channel computes its partner's convolution as well.
 template <typename T>
-__global__ void __launch_bounds__(256) group_prep_kernel(const msa_lm_group_args a) {
+__global__ void __launch_bounds__(256) group_prep_kernel(const msa_lm_group_args a, int first, int ring) {
   extern __shared__ float2 s_turn[];            // cosine and sine of the row's angles
   const GroupLayout L(a);
-  if ((int)blockIdx.x >= a.n_tok) { copy_old_row<T, 1>(a, L, (int)blockIdx.x - a.n_tok); return; }
+  if ((int)blockIdx.x >= a.n_tok) { copy_old_row<T, 1>(a, L, first, ring, (int)blockIdx.x - a.n_tok); return; }
   const long long n = blockIdx.x;
   const int s = a.tok_seq[n], t = (int)n - a.cu[s], p0 = a.start[s], pos = a.pos[n], slot = a.slot[s];
   for (int j = threadIdx.x; j < a.rot / 2; j += blockDim.x) {
@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(256) group_prep_kernel(const msa_lm_group_args
   __syncthreads();
   const ConvSource<T> src{reinterpret_cast<const T*>(a.proj), a.proj_stride, reinterpret_cast<T*>(a.conv_state), L.chan, a.taps};
   T* q = reinterpret_cast<T*>(a.q_out) + n * a.heads * a.q_pitch;
-  T* row = group_row<T>(a, L, n, s, t, p0);
+  T* row = group_row<T>(a, L, first, ring, n, s, t, p0);
   for (int c = threadIdx.x; c < L.chan; c += blockDim.x) {
     const GroupColumn g = group_column(a, L, c);
     float y = src.value(a.conv_w, n, t, p0, slot, c);
@@ -95,12 +95,12 @@ __global__ void __launch_bounds__(256) group_prep_kernel(const msa_lm_group_args
 
 // Four channels per thread, up to eight packed rows per block: every input is loaded once.
 template <typename T, int TAPS>
-__global__ void __launch_bounds__(256) group_prep_vec_kernel(const msa_lm_group_args a, int row_blocks, int rows) {
+__global__ void __launch_bounds__(256) group_prep_vec_kernel(const msa_lm_group_args a, int row_blocks, int rows, int first, int ring) {
   grid_dependency_wait();
   extern __shared__ float2 s_turn[];            // [rows][rot / 2]
   const GroupLayout L(a);
   if ((int)blockIdx.x >= row_blocks) {
-    if (blockIdx.y == 0) copy_old_row<T, 4>(a, L, (int)blockIdx.x - row_blocks);
+    if (blockIdx.y == 0) copy_old_row<T, 4>(a, L, first, ring, (int)blockIdx.x - row_blocks);
     return;
   }
   const int row0 = blockIdx.x * rows, n_here = min(rows, a.n_tok - row0), half = a.rot / 2;
@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(256) group_prep_vec_kernel(const msa_lm_group_
     const float2* turn = s_turn + r * half + (g.i >> 1);
     if (turns0) { const float2 cs = turn[0]; y = make_float4(y.x * cs.x - y.y * cs.y, y.y * cs.x + y.x * cs.y, y.z, y.w); }
     if (turns1) { const float2 cs = turn[1]; y = make_float4(y.x, y.y, y.z * cs.x - y.w * cs.y, y.w * cs.x + y.z * cs.y); }
-    T* dst = g.query ? reinterpret_cast<T*>(a.q_out) + n * a.heads * a.q_pitch : group_row<T>(a, L, n, s, t, p0);
+    T* dst = g.query ? reinterpret_cast<T*>(a.q_out) + n * a.heads * a.q_pitch : group_row<T>(a, L, first, ring, n, s, t, p0);
     store4(dst + g.at, y);
     if (n < a.n_decode) win.leave(src, slot, p0, c);
   }
@@ -163,6 +163,7 @@ struct GroupDecodeParams {
   const __nv_bfloat16* ring; long long ring_rows;
   const int32_t *slot, *pos;
   int heads, kv_heads, window, splits, sink;
+  int first;                        // tokens that stay visible
   float scale_log2e;
   const __nv_bfloat16* gate; long long gate_row;
   __nv_bfloat16* out; long long out_row;
@@ -185,12 +186,14 @@ __global__ void __launch_bounds__(kMmaWarps * 32, 2) group_decode_kernel(const G
   const int n_heads = min(kRows, G - g0), h0 = kvh * G + g0;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = lane >> 2, quad = lane & 3;
 
-  const int pos = p.pos[b], lo = max(0, pos - p.window + 1), total = pos - lo + 1;
+  // Visible rows in order: the first tokens in front of the window, then the window lo .. pos.
+  const int pos = p.pos[b], lo = max(0, pos - p.window + 1), front = min(p.first, lo), total = front + pos - lo + 1;
   int per = (total + p.splits - 1) / p.splits;
   per = (per + kMmaKeys - 1) / kMmaKeys * kMmaKeys;
   const int k0 = split * per, k1 = min(total, k0 + per);
   const int n_blocks = k1 > k0 ? (k1 - k0 + kMmaKeys - 1) / kMmaKeys : 0;
-  const int width = p.kv_heads * (D + DV), n_ring = (int)p.ring_rows, lo_row = lo % n_ring;
+  const int width = p.kv_heads * (D + DV), n_ring = (int)p.ring_rows, turn = n_ring - p.first;
+  const int lo_row = ring_row(lo, p.first, n_ring) - front;
   const __nv_bfloat16* ring = p.ring + (long long)p.slot[b] * p.ring_rows * width;
   const int k_col = kvh * D, v_col = p.kv_heads * D + kvh * DV;
 
@@ -208,8 +211,9 @@ __global__ void __launch_bounds__(kMmaWarps * 32, 2) group_decode_kernel(const G
     auto source = [&](int r, int col, bool& on) {
       const int k = k0 + blk * kMmaKeys + r;
       on = k < k1;
-      int at = lo_row + (on ? k : k0);                     // both terms are below the ring's size
-      at = at >= n_ring ? at - n_ring : at;
+      const int v = on ? k : k0;
+      int at = v < front ? v : lo_row + v;                 // below first + 2 * (ring rows - first)
+      at = at >= n_ring ? at - turn : at;
       return ring + (long long)at * width + col;
     };
 #pragma unroll
@@ -361,7 +365,9 @@ int launch_group_decode_any(const GroupDecodeParams& p, int n, cudaStream_t stre
 
 using namespace msa;
 
-extern "C" int msa_lm_group_prep(const msa_lm_group_args* args, void* stream) {
+extern "C" int msa_lm_group_prep(const msa_lm_group_args* args, void* stream) { return msa_lm_group_prep_first(args, 0, stream); }
+
+extern "C" int msa_lm_group_prep_first(const msa_lm_group_args* args, int32_t first, void* stream) {
   MSA_REQUIRE(args, "group_prep: null arguments");
   const msa_lm_group_args a = *args;
   MSA_REQUIRE(dtype_ok(a.dtype) && a.proj && a.conv_w && a.q_out && a.ring && a.pos && a.tok_seq && a.slot && a.start && a.cu,
@@ -372,9 +378,11 @@ extern "C" int msa_lm_group_prep(const msa_lm_group_args* args, void* stream) {
   MSA_REQUIRE(a.taps >= 1 && (a.taps == 1 || a.conv_state) && (a.rot == 0 || a.inv_freq), "group_prep: convolution state or angles missing");
   MSA_REQUIRE(a.n_decode >= 0 && a.n_decode <= a.n_seq && a.n_tok >= a.n_decode && a.n_old >= 0, "group_prep: bad counts");
   MSA_REQUIRE(a.n_seq == a.n_decode || (a.ctx && a.ctx_off && a.old_off), "group_prep: portions need a context");
+  MSA_REQUIRE(first_fits(first, a.window, a.ring_rows), "group_prep: the ring has no room for the first tokens and the window");
   if (a.n_tok == 0) return MSA_OK;
   cudaStream_t st = (cudaStream_t)stream;
   const GroupLayout L(a);
+  const int ring = ring_size(a.ring_rows);
   const int e4 = 4 * (int)dtype_size(a.dtype);
   auto ok4 = [&](const void* q) { return q == nullptr || reinterpret_cast<uintptr_t>(q) % e4 == 0; };
   const size_t turn = (size_t)a.rot * 4;         // a row's cosines and sines
@@ -384,19 +392,19 @@ extern "C" int msa_lm_group_prep(const msa_lm_group_args* args, void* stream) {
     const int rows = a.n_tok <= 256 ? 1 : kGpRows, row_blocks = (a.n_tok + rows - 1) / rows;
     const dim3 grid((unsigned)(row_blocks + a.n_old), (unsigned)((L.chan + 1023) / 1024));
     MSA_LM_DISPATCH(a.dtype, {
-      void (*kernel)(msa_lm_group_args, int, int);
+      void (*kernel)(msa_lm_group_args, int, int, int, int);
       switch (a.taps) {
         case 1: kernel = group_prep_vec_kernel<T, 1>; break;
         case 2: kernel = group_prep_vec_kernel<T, 2>; break;
         case 3: kernel = group_prep_vec_kernel<T, 3>; break;
         default: kernel = group_prep_vec_kernel<T, 4>;
       }
-      MSA_CUDA_OK(launch_kernel_pdl(kernel, grid, dim3(256), rows * turn, st, a.n_tok <= kEarlyRows, a, row_blocks, rows));
+      MSA_CUDA_OK(launch_kernel_pdl(kernel, grid, dim3(256), rows * turn, st, a.n_tok <= kEarlyRows, a, row_blocks, rows, first, ring));
     });
     MSA_LAUNCH_OK("group_prep_vec_kernel");
     return MSA_OK;
   }
-  MSA_LM_DISPATCH(a.dtype, { group_prep_kernel<T><<<a.n_tok + a.n_old, 256, turn, st>>>(a); });
+  MSA_LM_DISPATCH(a.dtype, { group_prep_kernel<T><<<a.n_tok + a.n_old, 256, turn, st>>>(a, first, ring); });
   MSA_LAUNCH_OK("group_prep_kernel");
   return MSA_OK;
 }
@@ -420,15 +428,24 @@ extern "C" int msa_lm_group_decode(const void* q, int64_t q_row, const void* rin
                                    const int32_t* pos, int32_t n, int32_t heads, int32_t kv_heads, int32_t dim, int32_t vdim,
                                    int32_t window, int32_t splits, float scale, int32_t sink, const void* gate, int64_t gate_row,
                                    void* out, int64_t out_row, float* part_o, float* part_ml, void* stream) {
+  return msa_lm_group_decode_first(q, q_row, ring, ring_rows, slot, pos, n, heads, kv_heads, dim, vdim, window, 0, splits, scale, sink, gate, gate_row,
+                                   out, out_row, part_o, part_ml, stream);
+}
+
+extern "C" int msa_lm_group_decode_first(const void* q, int64_t q_row, const void* ring, int64_t ring_rows, const int32_t* slot,
+                                         const int32_t* pos, int32_t n, int32_t heads, int32_t kv_heads, int32_t dim, int32_t vdim,
+                                         int32_t window, int32_t first, int32_t splits, float scale, int32_t sink, const void* gate,
+                                         int64_t gate_row, void* out, int64_t out_row, float* part_o, float* part_ml, void* stream) {
   MSA_REQUIRE(q && ring && slot && pos && out, "group_decode: null pointer");
   MSA_REQUIRE(msa_lm_group_decode_supported(dim, vdim) && heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && window > 0 &&
                   ring_rows > 0 && ring_rows < (1ll << 30), "group_decode: bad sizes");
+  MSA_REQUIRE(first_fits(first, window, ring_rows), "group_decode: the ring has no room for the first tokens and the window");
   MSA_REQUIRE(splits >= 1 && splits <= 64 && (splits == 1 || (part_o && part_ml)), "group_decode: bad splits");
   MSA_REQUIRE(aligned16(q) && aligned16(ring) && q_row % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 8 == 0 && out_row % 4 == 0 &&
                   (splits == 1 || (aligned16(part_o) && aligned16(part_ml))), "group_decode: alignment");
   if (n <= 0) return MSA_OK;
   const GroupDecodeParams p{(const __nv_bfloat16*)q, q_row, (const __nv_bfloat16*)ring, ring_rows, slot, pos, heads, kv_heads, window, splits,
-                            sink, scale * 1.4426950408889634f, (const __nv_bfloat16*)gate, gate_row, (__nv_bfloat16*)out, out_row, part_o, part_ml};
+                            sink, first, scale * 1.4426950408889634f, (const __nv_bfloat16*)gate, gate_row, (__nv_bfloat16*)out, out_row, part_o, part_ml};
   cudaStream_t st = (cudaStream_t)stream;
   if (dim == 64) return vdim == 64 ? launch_group_decode_any<64, 64>(p, n, st) : launch_group_decode_any<64, 128>(p, n, st);
   return vdim == 64 ? launch_group_decode_any<128, 64>(p, n, st) : launch_group_decode_any<128, 128>(p, n, st);

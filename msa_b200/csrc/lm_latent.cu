@@ -145,14 +145,14 @@ __global__ void __launch_bounds__(128) latent_prep_vec_kernel(const LatentPrepPa
 template <typename T>
 __global__ void __launch_bounds__(128)
 ring_store_kernel(const T* __restrict__ ctx, int width, const int32_t* slot, const int32_t* start, const int32_t* cu,
-                  const int32_t* ctx_off, int n_decode, int window, T* ring, long long ring_rows) {
+                  const int32_t* ctx_off, int n_decode, int window, int first, T* ring, long long ring_rows, int rows) {
   const int ps = blockIdx.y, s = ps + n_decode;
   const int len = cu[s + 1] - cu[s], p0 = start[s];
-  const int keep = (int)min((long long)len, ring_rows);
-  for (int k = blockIdx.x; k < keep; k += gridDim.x) {
-    const int t = len - keep + k;
-    const T* src = ctx + (long long)(ctx_off[ps] + min(p0, window - 1) + t) * width;
-    T* dst = ring + ((long long)slot[s] * ring_rows + (p0 + t) % ring_rows) * width;
+  const int front = max(0, min(first - p0, len)), tail = max(front, len - (rows - first));   // tokens that are first ones; from `tail` on: kept last ones
+  for (int k = blockIdx.x; k < front + len - tail; k += gridDim.x) {
+    const int t = k < front ? k : tail + k - front;
+    const T* src = ctx + (long long)(ctx_off[ps] + old_rows(p0, first + window) + t) * width;
+    T* dst = ring + ((long long)slot[s] * ring_rows + ring_row(p0 + t, first, rows)) * width;
     for (int i = threadIdx.x; i < width; i += blockDim.x) dst[i] = src[i];
   }
 }
@@ -162,7 +162,7 @@ ring_store_kernel(const T* __restrict__ ctx, int width, const int32_t* slot, con
 // memory as fp32; lane = key for the scores, lane = value column for the output.
 constexpr int kGaRows = 8, kGaThreads = 128;
 
-__global__ void __launch_bounds__(kGaThreads) window_attn_kernel(const msa_lm_attn_args a, int heads_per_block, int tile) {
+__global__ void __launch_bounds__(kGaThreads) window_attn_kernel(const msa_lm_attn_args a, int heads_per_block, int tile, int n_first, int ring) {
   extern __shared__ float sm[];
   const int dq = a.da + a.db, kstr = dq + 1;
   float* s_q = sm;                         // [8][dq]
@@ -188,16 +188,18 @@ __global__ void __launch_bounds__(kGaThreads) window_attn_kernel(const msa_lm_at
   const int t_lo = (int)(r0 / hg), t_hi = (int)((r0 + nr - 1) / hg);
   const int p_lo = start + t_lo, p_hi = start + t_hi;
   const int j0 = max(0, p_lo - a.window + 1);
-  const int first = start - min(start, a.window - 1);
+  const int front = min(n_first, j0);                                     // first tokens in front of the window
+  const int gap = start - old_rows(start, n_first + a.window);            // positions that the context leaves out behind the first tokens
   const float m0 = a.sink ? 0.f : -INFINITY, l0 = a.sink ? 1.f : 0.f;     // the sink: one entry with score 0 and no value
   float m[2] = {m0, m0}, l[2] = {l0, l0};
-  for (int jt = j0; jt <= p_hi; jt += tile) {
-    const int nk = min(tile, p_hi - jt + 1);
+  const int n_keys = front + p_hi - j0 + 1;
+  for (int kt = 0; kt < n_keys; kt += tile) {
+    const int nk = min(tile, n_keys - kt);
     __syncthreads();
     for (int i = threadIdx.x; i < nk * (dq + a.dv); i += kGaThreads) {
-      const int k = i / (dq + a.dv), c = i % (dq + a.dv), j = jt + k;
-      const long long row = a.ring_rows > 0 ? (long long)a.slot[s] * a.ring_rows + j % a.ring_rows
-                                            : (long long)a.ctx_off[s - a.seq0] + (j - first);
+      const int k = i / (dq + a.dv), c = i % (dq + a.dv), j = kt + k < front ? kt + k : j0 - front + kt + k;
+      const long long row = a.ring_rows > 0 ? (long long)a.slot[s] * a.ring_rows + ring_row(j, n_first, ring)
+                                            : (long long)a.ctx_off[s - a.seq0] + (j < n_first ? j : j - gap);
       if (c < a.da) s_k[k * kstr + c] = load_any(a.ka, a.dtype, row * a.ka_row + blockIdx.y * a.ka_head + c);
       else if (c < dq) s_k[k * kstr + c] = load_any(a.kb, a.dtype, row * a.kb_row + blockIdx.y * a.kb_head + (c - a.da));
       else s_v[k * a.dv + (c - dq)] = load_any(a.v, a.dtype, row * a.v_row + blockIdx.y * a.v_head + (c - dq));
@@ -207,9 +209,9 @@ __global__ void __launch_bounds__(kGaThreads) window_attn_kernel(const msa_lm_at
     for (int q = 0; q < 2; ++q) {
       const int r = warp * 2 + q;
       if (r >= nr) continue;
-      const int pos = start + (int)((r0 + r) / hg), j = jt + lane;
+      const int pos = start + (int)((r0 + r) / hg), j = kt + lane < front ? kt + lane : j0 - front + kt + lane;
       float sc = -INFINITY;
-      if (lane < nk && j <= pos && pos - j < a.window) {
+      if (lane < nk && j <= pos && (pos - j < a.window || j < n_first)) {
         float acc = 0.f;
         for (int c = 0; c < dq; ++c) acc = fmaf(s_q[r * dq + c], s_k[lane * kstr + c], acc);
         sc = acc * a.scale;
@@ -279,26 +281,36 @@ extern "C" int msa_lm_latent_prep(void* proj, int64_t proj_stride, const float* 
 extern "C" int msa_lm_ring_store(const void* ctx, int32_t row_width, const int32_t* slot, const int32_t* start,
                                  const int32_t* cu, const int32_t* ctx_off, int32_t n_seq, int32_t n_decode, int32_t max_len,
                                  int32_t window, void* ring, int64_t ring_rows, int32_t dtype, void* stream) {
+  return msa_lm_ring_store_first(ctx, row_width, slot, start, cu, ctx_off, n_seq, n_decode, max_len, window, 0, ring, ring_rows, dtype, stream);
+}
+
+extern "C" int msa_lm_ring_store_first(const void* ctx, int32_t row_width, const int32_t* slot, const int32_t* start,
+                                       const int32_t* cu, const int32_t* ctx_off, int32_t n_seq, int32_t n_decode, int32_t max_len,
+                                       int32_t window, int32_t first, void* ring, int64_t ring_rows, int32_t dtype, void* stream) {
   MSA_REQUIRE(dtype_ok(dtype) && ctx && slot && start && cu && ctx_off && ring && row_width > 0 && ring_rows > 0,
               "ring_store: bad arguments");
+  MSA_REQUIRE(first_fits(first, window, ring_rows), "ring_store: the ring has no room for the first tokens and the window");
   if (n_seq <= n_decode || max_len <= 0) return MSA_OK;
   const int64_t rows = max_len < ring_rows ? max_len : ring_rows;
   const dim3 grid((unsigned)(rows < 4096 ? rows : 4096), (unsigned)(n_seq - n_decode));
   MSA_LM_DISPATCH(dtype, {
     ring_store_kernel<T><<<grid, 128, 0, (cudaStream_t)stream>>>((const T*)ctx, row_width, slot, start, cu, ctx_off, n_decode,
-                                                                window, (T*)ring, ring_rows);
+                                                                window, first, (T*)ring, ring_rows, ring_size(ring_rows));
   });
   MSA_LAUNCH_OK("ring_store_kernel");
   return MSA_OK;
 }
 
-extern "C" int msa_lm_window_attn(const msa_lm_attn_args* args, void* stream) {
+extern "C" int msa_lm_window_attn(const msa_lm_attn_args* args, void* stream) { return msa_lm_window_attn_first(args, 0, stream); }
+
+extern "C" int msa_lm_window_attn_first(const msa_lm_attn_args* args, int32_t first, void* stream) {
   MSA_REQUIRE(args, "window_attn: null arguments");
   const msa_lm_attn_args a = *args;
   MSA_REQUIRE(dtype_ok(a.dtype) && dtype_ok(a.qa_dtype) && dtype_ok(a.out_dtype), "window_attn: bad dtype");
   MSA_REQUIRE(a.qa && a.ka && a.v && a.out && a.start && a.cu && (a.db == 0 || (a.qb && a.kb)), "window_attn: null pointer");
   MSA_REQUIRE(a.ring_rows > 0 ? a.slot != nullptr : a.ctx_off != nullptr, "window_attn: no key addressing");
   MSA_REQUIRE(a.heads > 0 && a.da > 0 && a.db >= 0 && a.dv > 0 && a.window > 0, "window_attn: bad sizes");
+  MSA_REQUIRE(first_fits(first, a.window, a.ring_rows), "window_attn: the ring has no room for the first tokens and the window");
   if (a.seq1 <= a.seq0 || a.max_len <= 0) return MSA_OK;
   MSA_REQUIRE(a.group > 0 && a.heads % a.group == 0, "window_attn: heads must be a multiple of group");
   const int hg = a.group;
@@ -311,7 +323,7 @@ extern "C" int msa_lm_window_attn(const msa_lm_attn_args* args, void* stream) {
   MSA_OK_OR_RETURN(ensure_dynamic_smem(window_attn_kernel, bytes(tile), state));
   const dim3 grid((unsigned)(((long long)a.max_len * hg + kGaRows - 1) / kGaRows), (unsigned)(a.heads / hg),
                   (unsigned)(a.seq1 - a.seq0));
-  window_attn_kernel<<<grid, kGaThreads, bytes(tile), (cudaStream_t)stream>>>(a, hg, tile);
+  window_attn_kernel<<<grid, kGaThreads, bytes(tile), (cudaStream_t)stream>>>(a, hg, tile, first, ring_size(a.ring_rows));
   MSA_LAUNCH_OK("window_attn_kernel");
   return MSA_OK;
 }

@@ -163,7 +163,7 @@ class GatedDelta(Mixer):
 
 def portion_attention(args, tc: bool, status, step, view, scale, **kw) -> None:
     """The portions of a step (``args``: q parts, k parts, v, out) over their packed context."""
-    kw.update(scale=scale, window=view.window, start=step.start, cu=step.cu, seq0=step.n_decode, seq1=step.n_seq, max_len=step.max_len,
+    kw.update(scale=scale, window=view.window, first=view.first, start=step.start, cu=step.cu, seq0=step.n_decode, seq1=step.n_seq, max_len=step.max_len,
               ctx_off=view.ctx_off)
     if tc:
         K.window_attn_tc(*args, row0=step.n_decode, status=status, **kw)
@@ -172,7 +172,7 @@ def portion_attention(args, tc: bool, status, step, view, scale, **kw) -> None:
 
 
 class GroupedAttention(Mixer):
-    """Grouped-query window attention behind a short convolution, with a silent sink and a gate per head.  Head sizes up to 128
+    """Grouped-query window attention behind a short convolution, with first tokens that stay visible, a silent sink and a gate per head.  Head sizes up to 128
     are stored with zeros up to 64 or 128 in bf16, so that the tensor-core kernels take any of them."""
 
     def __init__(self, spec, w: Weights, prefix: str, width: int, eps: float):
@@ -194,14 +194,14 @@ class GroupedAttention(Mixer):
     @property
     def state_spec(self) -> RingSpec:
         s = self.spec
-        return RingSpec(s.kv_heads * (self.dim + self.vdim), s.window, s.channels, s.taps)
+        return RingSpec(s.kv_heads * (self.dim + self.vdim), s.window, s.channels, s.taps, s.first)
 
     def forward(self, h, step, cache, run, out=None):
         return self.mix(K.matmul(h, self.w_in, weight=True), step, cache, run, out)
 
     def mix(self, proj: torch.Tensor, step, cache: SequenceStateCache, run: int, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         s, n, nd = self.spec, step.n_tok, step.n_decode
-        ring, view, conv = cache.ring[run], step.views[s.window], cache.conv[run]
+        ring, view, conv = cache.ring[run], step.views[s.span], cache.conv[run]
         new = torch.empty if (self.dim, self.vdim) == (s.dim, s.vdim) else torch.zeros      # the filling must be zero
         kw = dict(dtype=proj.dtype, device=proj.device)
         q = new((n, s.heads, self.dim), **kw)
@@ -214,11 +214,11 @@ class GroupedAttention(Mixer):
         split = s.kv_heads * self.dim
         parts = lambda rows: (rows[:, :split].unflatten(1, (s.kv_heads, self.dim)), rows[:, split:].unflatten(1, (s.kv_heads, self.vdim)))
         if nd and self.tc_decode:
-            K.group_decode(q[:nd], ring, s.kv_heads, step, heads_out[:nd], window=view.window, scale=s.scale, sink=s.sink,
+            K.group_decode(q[:nd], ring, s.kv_heads, step, heads_out[:nd], window=view.window, first=view.first, scale=s.scale, sink=s.sink,
                            gate=None if gate is None else gate[:nd])
         elif nd:
             k, v = parts(ring.view(-1, ring.shape[2]))
-            K.window_attn(q[:nd], None, k, None, v, heads_out[:nd], scale=s.scale, window=view.window, start=step.start, cu=step.cu, seq0=0,
+            K.window_attn(q[:nd], None, k, None, v, heads_out[:nd], scale=s.scale, window=view.window, first=view.first, start=step.start, cu=step.cu, seq0=0,
                           seq1=nd, max_len=1, slot=step.slot, ring_rows=ring.shape[1], sink=s.sink, gate=None if gate is None else gate[:nd])
         if n > nd:
             K.conv_store(proj, s.channels, s.taps, step, conv)

@@ -31,6 +31,8 @@ class LatentAttentionSpec:
         if rot.get("dims", m["rot_dim"]) != m["rot_dim"]:
             raise ValueError(f"latent_attention: rot.dims {rot['dims']} differs from rot_dim {m['rot_dim']}")
         mask = m.get("mask") or {}
+        if mask.get("first"):
+            raise ValueError("latent_attention: first tokens that stay visible (mask.first) are for attention layers")
         return cls(heads=int(m["heads"]), dim=int(m["dim"]), rot_dim=int(m["rot_dim"]), vdim=int(m["vdim"]),
                    kv_rank=int(m["kv_rank"]), scale=float(m["scale"]), rot_base=float(rot["base"]),
                    window=int(mask["size"]) if mask.get("size") is not None else None)
@@ -64,7 +66,8 @@ class DeltaSpec:
 class GroupedAttentionSpec:
     """Grouped-query attention over a sliding window, queries, keys and values behind a short causal convolution of ``taps``
     taps; the first ``rot_dims`` dimensions of a head are rotated (neighbouring pairs).  ``sink``: one is added to the
-    softmax denominators; ``gate``: every head's output is multiplied by the sigmoid of a projection of the layer's input."""
+    softmax denominators; ``gate``: every head's output is multiplied by the sigmoid of a projection of the layer's input; ``first``
+    tokens of a sequence stay visible when the window has moved on."""
     heads: int
     kv_heads: int
     dim: int
@@ -76,6 +79,7 @@ class GroupedAttentionSpec:
     taps: int
     sink: bool = True
     gate: bool = True
+    first: int = 0
 
     kind = "attention"
 
@@ -84,7 +88,9 @@ class GroupedAttentionSpec:
         rot, mask = m.get("rot") or {"dims": 0, "base": 1.0}, m.get("mask") or {}
         spec = cls(heads=int(m["heads"]), kv_heads=int(m["kv_heads"]), dim=int(m["dim"]), vdim=int(m["vdim"]), scale=float(m["scale"]),
                    rot_dims=int(rot["dims"]), rot_base=float(rot["base"]), taps=int(m["conv"]),
-                   window=int(mask["size"]) if mask.get("size") is not None else None)
+                   window=int(mask["size"]) if mask.get("size") is not None else None, first=int(mask.get("first") or 0))
+        if spec.first < 0:
+            raise ValueError(f"attention: {spec.first} first tokens")
         if spec.heads % spec.kv_heads:
             raise ValueError(f"attention: {spec.heads} heads are not a multiple of {spec.kv_heads} kv_heads")
         if spec.rot_dims % 2 or not 0 <= spec.rot_dims <= spec.dim:
@@ -94,6 +100,11 @@ class GroupedAttentionSpec:
     @property
     def channels(self) -> int:
         return (self.heads + self.kv_heads) * self.dim + self.kv_heads * self.vdim
+
+    @property
+    def span(self):
+        """The window as steps and caches name it."""
+        return self.window if self.window is None or not self.first else (self.window, self.first)
 
 
 @dataclass(frozen=True)
@@ -271,10 +282,12 @@ class HybridConfig:
         return len(self.runs())
 
     @property
-    def windows(self) -> Tuple[Optional[int], ...]:
-        """The distinct attention windows, in order of appearance."""
-        out: List[Optional[int]] = []
+    def windows(self) -> Tuple[Union[None, int, Tuple[int, int]], ...]:
+        """The distinct attention windows, in order of appearance: a size, or (size, first tokens that stay visible)."""
+        out: List[Union[None, int, Tuple[int, int]]] = []
         for layer in self.layers:
-            if hasattr(layer.mixer, "window") and layer.mixer.window not in out:
-                out.append(layer.mixer.window)
+            if hasattr(layer.mixer, "window"):
+                span = getattr(layer.mixer, "span", layer.mixer.window)
+                if span not in out:
+                    out.append(span)
         return tuple(out)

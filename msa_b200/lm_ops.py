@@ -191,8 +191,8 @@ def latent_prep(proj, spec, w_norm, inv_freq, eps, step, view, ring, ctx):
 
 
 def ring_store(ctx, step, view, ring):
-    A.call("msa_lm_ring_store", A.ptr(ctx), ctx.shape[1], A.ptr(step.slot), A.ptr(step.start), A.ptr(step.cu),
-           A.ptr(view.ctx_off), step.n_seq, step.n_decode, step.max_len, view.window, A.ptr(ring), ring.shape[1],
+    A.call("msa_lm_ring_store_first", A.ptr(ctx), ctx.shape[1], A.ptr(step.slot), A.ptr(step.start), A.ptr(step.cu),
+           A.ptr(view.ctx_off), step.n_seq, step.n_decode, step.max_len, view.window, view.first, A.ptr(ring), ring.shape[1],
            A.dtype_code(ctx.dtype), A.stream_ptr(ctx.device))
 
 
@@ -215,19 +215,19 @@ def attn_args(qa, qb, ka, kb, v, out, *, scale, window, start, cu, seq0, seq1, m
         qa_dtype=A.dtype_code(qa.dtype), out_dtype=A.dtype_code(out.dtype), dtype=A.dtype_code(ka.dtype), scale=float(scale))
 
 
-def window_attn(qa, qb, ka, kb, v, out, **kw):
-    """General windowed attention (any sizes, both dtypes)."""
-    A.call("msa_lm_window_attn", C.byref(attn_args(qa, qb, ka, kb, v, out, **kw)), A.stream_ptr(qa.device))
+def window_attn(qa, qb, ka, kb, v, out, *, first=0, **kw):
+    """General windowed attention (any sizes, both dtypes); ``first``: tokens that stay visible in front of the window."""
+    A.call("msa_lm_window_attn_first", C.byref(attn_args(qa, qb, ka, kb, v, out, **kw)), first, A.stream_ptr(qa.device))
 
 
 def window_attn_tc_supported(dim, rot, vdim, dtype, scale) -> bool:
     return dtype == torch.bfloat16 and scale > 0 and bool(A.lib().msa_lm_window_attn_tc_supported(dim, rot, vdim))
 
 
-def window_attn_tc(qa, qb, ka, kb, v, out, *, row0, status, **kw):
+def window_attn_tc(qa, qb, ka, kb, v, out, *, row0, status, first=0, **kw):
     """The portions of a step on the tensor cores: ``qa`` / ``out`` from the first portion row (packed row ``row0``) on."""
     args = attn_args(qa, qb, ka, kb, v, out, **kw)
-    A.call("msa_lm_window_attn_tc", C.byref(args), qa.shape[0], ka.shape[0], row0, A.ptr(status), A.stream_ptr(qa.device))
+    A.call("msa_lm_window_attn_tc_first", C.byref(args), first, qa.shape[0], ka.shape[0], row0, A.ptr(status), A.stream_ptr(qa.device))
 
 
 def latent_decode_supported(spec, dtype) -> bool:
@@ -264,7 +264,7 @@ def group_prep(proj, spec, w, step, view, ring, conv_state, q, ctx):
                        ring_rows=ring.shape[1], heads=spec.heads, kv_heads=spec.kv_heads, dim=spec.dim, vdim=spec.vdim, rot=spec.rot_dims,
                        taps=spec.taps, q_pitch=w.dim, k_pitch=w.dim, v_pitch=w.vdim, n_tok=step.n_tok, n_seq=step.n_seq,
                        n_decode=step.n_decode, n_old=view.n_old, window=view.window, dtype=A.dtype_code(proj.dtype))
-    A.call("msa_lm_group_prep", C.byref(args), A.stream_ptr(proj.device))
+    A.call("msa_lm_group_prep_first", C.byref(args), view.first, A.stream_ptr(proj.device))
 
 
 def conv_store(proj, channels, taps, step, conv_state):
@@ -285,8 +285,9 @@ def group_decode_splits(n: int, heads: int, kv_heads: int, ring_rows: int, n_sm:
     return max(1, min(2 * n_sm // max(n * tiles, 1), (ring_rows + 63) // 64, 64))
 
 
-def group_decode(q, ring, kv_heads, step, out, *, window, scale, sink, gate):
-    """``q`` [n, heads, dim], ``out`` [n, heads, vdim] views, ``ring`` [slots, rows, kv_heads * (dim + vdim)]."""
+def group_decode(q, ring, kv_heads, step, out, *, window, scale, sink, gate, first=0):
+    """``q`` [n, heads, dim], ``out`` [n, heads, vdim] views, ``ring`` [slots, rows, kv_heads * (dim + vdim)]; ``first``: tokens that
+    stay visible in front of the window."""
     n, heads, dim = q.shape
     vdim = out.shape[2]
     splits = group_decode_splits(n, heads, kv_heads, ring.shape[1])
@@ -294,8 +295,8 @@ def group_decode(q, ring, kv_heads, step, out, *, window, scale, sink, gate):
     if splits > 1:
         f = dict(dtype=torch.float32, device=q.device)
         part_o, part_ml = torch.empty((n, heads, splits, vdim), **f), torch.empty((n, heads, splits, 2), **f)
-    A.call("msa_lm_group_decode", A.ptr(q), q.stride(0), A.ptr(ring), ring.shape[1], A.ptr(step.slot), A.ptr(step.start), n, heads, kv_heads, dim,
-           vdim, window, splits, float(scale), 1 if sink else 0, A.ptr(gate), gate.stride(0) if gate is not None else 0, A.ptr(out),
+    A.call("msa_lm_group_decode_first", A.ptr(q), q.stride(0), A.ptr(ring), ring.shape[1], A.ptr(step.slot), A.ptr(step.start), n, heads, kv_heads, dim,
+           vdim, window, first, splits, float(scale), 1 if sink else 0, A.ptr(gate), gate.stride(0) if gate is not None else 0, A.ptr(out),
            out.stride(0), A.ptr(part_o), A.ptr(part_ml), A.stream_ptr(q.device))
 
 

@@ -43,10 +43,10 @@ def rotate_interleaved(x, positions, base):
     return out
 
 
-def window_mask(n, size):
-    """[n, n] boolean: row i may look at column j."""
+def window_mask(n, size, first=0):
+    """[n, n] boolean: row i may look at column j; the first ``first`` columns stay visible."""
     d = torch.arange(n)[:, None] - torch.arange(n)[None, :]
-    return (d >= 0) if size is None else (d >= 0) & (d < size)
+    return (d >= 0) if size is None else (d >= 0) & ((d < size) | (torch.arange(n)[None, :] < first))
 
 
 def latent_attention(h, w, spec, eps):
@@ -164,7 +164,8 @@ def softmax_plus_one(score):
 
 
 def window_attention(h, w, spec, eps=None):
-    """Grouped-query attention over a sliding window behind a short convolution, with a silent sink and one gate per head."""
+    """Grouped-query attention over a sliding window (and first tokens that stay visible) behind a short convolution, with a
+    silent sink and one gate per head."""
     n, heads, groups, dim, vdim = h.shape[0], spec["heads"], spec["kv_heads"], spec["dim"], spec["vdim"]
     pos, rot = torch.arange(n), spec.get("rot") or {"base": 1.0, "dims": 0}
     q, k, v = (causal_conv(h @ w[s].T, w[s + ".conv"]) for s in "qkv")
@@ -173,7 +174,7 @@ def window_attention(h, w, spec, eps=None):
     owner = torch.arange(heads) // (heads // groups)
     k, v = k[:, owner], v.view(n, groups, vdim)[:, owner]
     score = torch.einsum("ihd,jhd->hij", q, k) * spec["scale"]
-    mask = window_mask(n, (spec.get("mask") or {}).get("size"))
+    mask = window_mask(n, (spec.get("mask") or {}).get("size"), (spec.get("mask") or {}).get("first") or 0)
     o = torch.einsum("hij,jhd->ihd", softmax_plus_one(score.masked_fill(~mask, float("-inf"))), v)
     return (o * sigmoid(h @ w["g"].T)[:, :, None]).reshape(n, heads * vdim) @ w["o"].T
 
