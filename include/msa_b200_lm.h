@@ -321,6 +321,38 @@ typedef struct {
 } msa_lm_rows_gemm_args;
 int msa_lm_rows_gemm(const msa_lm_rows_gemm_args* args, void* stream);
 
+/* ---- beam search ----------------------------------------------------------------------------------------------------
+ * The k best continuations of every question's beams.  Row q * beams + b of logits [batch * beams, vocab] (stride elements
+ * apart) belongs to beam b, whose score is scores[q, b]; continuation (b, t) has the score scores[q, b] + x_t - log sum exp x, and
+ * score / beam / token [batch, k] receive the best in descending 64-bit order; equals: the lower beam, the larger logit, the lower token.  Logits of
+ * -inf are no continuations; neither are those of a beam whose score is not finite or whose row holds a NaN or +inf.  Places left over:
+ * (-inf, -1, -1).  live_* [batch, beams] (all or none): the first `beams` of the k whose token is not among stop [n_stop].
+ * 1 to 32 beams, k up to 64; workspace: msa_lm_beam_topk_workspace bytes, 8-byte aligned. */
+int64_t msa_lm_beam_topk_workspace(int32_t batch, int32_t beams, int32_t vocab, int32_t k);
+int msa_lm_beam_topk(const void* logits, int64_t stride, int32_t dtype, const float* scores, int32_t batch, int32_t beams, int32_t vocab,
+                     int32_t k, const int32_t* stop, int32_t n_stop, void* workspace, float* score, int32_t* beam, int32_t* token,
+                     float* live_score, int32_t* live_beam, int32_t* live_token, void* stream);
+
+/* What one tensor holds for a slot (slot_bytes apart from `base` on): all of its `bytes`; a ring of `rows` rows of `bytes` (the first `first`
+ * positions in front, see above); or two halves of `bytes`, of which the one of the next position's parity counts.  align: bytes that
+ * divide base, slot_bytes and bytes (16, 4 or 2). */
+enum { MSA_LM_STATE_ALL = 0, MSA_LM_STATE_RING = 1, MSA_LM_STATE_HALF = 2 };
+typedef struct {
+  void* base;
+  int64_t slot_bytes, bytes, rows;
+  int32_t first, kind, align, reserved;
+} msa_lm_state_part;
+/* Beam j of question q goes on from beam parent[q, j], with the state in slot[q, parent[q, j]], which holds length[q] positions: the
+ * first that names a parent keeps its slot, the others (and those with a parent outside 0 .. beams-1, which get no state) take, in
+ * order, the slots of beams that nobody names.  slot_out [batch, beams]: the new table.  parts [n_part] (device memory): the
+ * tensors.  shared [batch, beams, beams] (may be null): positions from the start on whose ring rows two beams' slots hold alike;
+ * those are not copied; shared_out the same for the new beams.  slot: distinct, below n_slots (a copy to or from others is left out).
+ * workspace: msa_lm_reorder_workspace bytes, 16-byte aligned. */
+int64_t msa_lm_reorder_workspace(int32_t batch, int32_t beams, int32_t n_part);
+int msa_lm_reorder(const int32_t* slot, const int32_t* parent, const int32_t* length, const int32_t* shared, int32_t batch, int32_t beams,
+                   int32_t n_slots, const msa_lm_state_part* parts, int32_t n_part, int32_t* slot_out, int32_t* shared_out, void* workspace,
+                   void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -2,6 +2,7 @@
 designs.  No fallback: a missing library or a failed call raises."""
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import os
 
@@ -19,7 +20,8 @@ EXPORTS = ["msa_lm_residual_norm", "msa_lm_embed", "msa_lm_silu_mul", "msa_lm_so
            "msa_lm_window_attn", "msa_lm_window_attn_tc_supported", "msa_lm_window_attn_tc", "msa_lm_latent_decode_supported", "msa_lm_latent_decode", "msa_lm_delta_decode", "msa_lm_delta_prep", "msa_lm_delta_prep_split", "msa_lm_delta_chunk_supported", "msa_lm_delta_chunk_workspace", "msa_lm_delta_chunk", "msa_lm_gather_rows", "msa_lm_delta_conv_store", "msa_lm_delta_scan",
            "msa_lm_delta_out", "msa_lm_moe_topk", "msa_lm_moe_sort", "msa_lm_moe_gemm", "msa_lm_moe_gemm_tc",
            "msa_lm_rows_gemm", "msa_lm_argmax", "msa_lm_group_prep_first", "msa_lm_ring_store_first", "msa_lm_window_attn_first",
-           "msa_lm_window_attn_tc_first", "msa_lm_group_decode_first"]
+           "msa_lm_window_attn_tc_first", "msa_lm_group_decode_first", "msa_lm_beam_topk_workspace", "msa_lm_beam_topk",
+           "msa_lm_reorder_workspace", "msa_lm_reorder"]
 
 vp, i32, i64, f32 = C.c_void_p, C.c_int32, C.c_int64, C.c_float
 
@@ -81,6 +83,13 @@ class RowsGemmArgs(C.Structure):
                 ("act", i32), ("early", i32), ("out_dtype", i32)]
 
 
+class StatePart(C.Structure):
+    """``msa_lm_state_part``."""
+    _fields_ = [("base", vp), ("slot_bytes", i64), ("bytes", i64), ("rows", i64), ("first", i32), ("kind", i32), ("align", i32), ("reserved", i32)]
+
+
+STATE_ALL, STATE_RING, STATE_HALF = 0, 1, 2
+
 _lib = None
 
 
@@ -128,6 +137,10 @@ def lib() -> C.CDLL:
             "msa_lm_window_attn_first": [ap, i32, vp],
             "msa_lm_window_attn_tc_first": [ap, i32, i32, i32, i32, vp, vp],
             "msa_lm_group_decode_first": [vp, i64, vp, i64, vp, vp, i32, i32, i32, i32, i32, i32, i32, i32, f32, i32, vp, i64, vp, i64, vp, vp, vp],
+            "msa_lm_beam_topk_workspace": [i32, i32, i32, i32],
+            "msa_lm_beam_topk": [vp, i64, i32, vp, i32, i32, i32, i32, vp, i32, vp, vp, vp, vp, vp, vp, vp, vp],
+            "msa_lm_reorder_workspace": [i32, i32, i32],
+            "msa_lm_reorder": [vp, vp, vp, vp, i32, i32, i32, vp, i32, vp, vp, vp, vp],
             "msa_lm_latent_decode_supported": [i32, i32],
             "msa_lm_latent_decode": [vp, i64, i64, vp, i64, i64, vp, i64, vp, vp, i32, i32, i32, i32, i32, i32, f32, vp, vp, vp, vp, vp],
             "msa_lm_moe_gemm_tc": [vp, i64, i32, vp, vp, i32, vp, vp, i32, i32, i32, i32, f32, vp, i64, vp, vp],
@@ -151,6 +164,11 @@ def lib() -> C.CDLL:
             getattr(l, name).restype = i64 if name.endswith("_workspace") else C.c_int
         _lib = l
     return _lib
+
+
+def on_device(device: torch.device):
+    """Makes ``device`` the current one for a launch, if it is not."""
+    return contextlib.nullcontext() if device.index in (None, torch.cuda.current_device()) else torch.cuda.device(device)
 
 
 launches = 0    # calls into the library since import (each is one kernel launch)

@@ -138,6 +138,9 @@ class SequenceStateCache(SparseCache):
         self._free: List[int] = list(range(n_slots - 1, -1, -1))
         self._slot: Dict[Hashable, int] = {}
         self._length: Dict[Hashable, int] = {}
+        self._parts: Optional[torch.Tensor] = None
+        if self.device.type == "cuda":
+            self._state_parts()              # here, so that a first ``reorder`` may be captured
 
     @property
     def free_slots(self) -> int:
@@ -166,6 +169,61 @@ class SequenceStateCache(SparseCache):
 
     def advance(self, seq: Hashable, n: int) -> None:
         self._length[seq] += n
+
+    def _state_parts(self) -> torch.Tensor:
+        """What a slot holds, tensor by tensor, for the kernels (``msa_lm_state_part``): device memory, made once."""
+        if self._parts is None:
+            from . import _cabi_lm as A
+            parts = []
+
+            def add(t: torch.Tensor, kind: int, unit: int, rows: int = 0, first: int = 0):
+                slot = t.stride(0) * t.element_size()
+                if unit and t.shape[0]:
+                    align = next(a for a in (16, 4, 2) if not (t.data_ptr() % a or slot % a or unit % a))
+                    parts.append(A.StatePart(t.data_ptr(), slot, unit, rows, first, kind, align, 0))
+            for i, s in enumerate(self.specs):
+                if i in self.ring:
+                    t = self.ring[i]
+                    add(t, A.STATE_RING, t.shape[2] * t.element_size(), t.shape[1], window_of((s.window, s.first), self.max_len)[1])
+                if i in self.conv:
+                    add(self.conv[i], A.STATE_HALF, self.conv[i][0, 0].numel() * self.conv[i].element_size())
+                for d in (self.state, self.shift):
+                    if i in d:
+                        add(d[i], A.STATE_ALL, d[i][0].numel() * d[i].element_size())
+            add(self.last_token, A.STATE_ALL, self.last_token.element_size())
+            raw = torch.frombuffer(bytearray(b"".join(bytes(p) for p in parts)), dtype=torch.int64).view(len(parts), -1)
+            self._parts = raw.to(self.device)
+        return self._parts
+
+    def reorder(self, slot: torch.Tensor, parent: torch.Tensor, length: torch.Tensor, shared: Optional[torch.Tensor] = None
+                ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+        """Beam j of question q goes on from beam ``parent[q, j]``: returns the new table of slots and the new ``shared`` (None without).
+
+        ``slot`` ``[batch, beams]``: the slots the beams held (distinct, of ``acquire``); ``length`` ``[batch]``: the positions in them.  The
+        first beam that names a parent keeps its slot; the others take, in order, the slots that nobody continues, and the parent's
+        state is copied there, in every run.  A parent of -1 names nobody: such a beam gets a slot, but no state.  ``shared``
+        ``[batch, beams, beams]``: positions from the start on whose ring rows two beams' slots hold alike (zeros when beams begin,
+        then what the last call returned, as long as the slots advance by nothing but the beams' own tokens); those rows are not
+        copied.  All int32 on the cache's device; 1 to 32 beams.  Runs in the current stream, nothing is read back; the bookkeeping
+        by sequence (``slot(seq)``) stays as it was."""
+        from . import _cabi_lm as A
+        A.need_cuda(slot, parent, length, shared)
+        if slot.dim() != 2 or not 1 <= slot.shape[1] <= 32:
+            raise A.MsaError(f"reorder: slots [batch, 1 to 32 beams] expected, not {tuple(slot.shape)}")
+        batch, beams = slot.shape
+        if parent.shape != slot.shape or length.shape != (batch,) or (shared is not None and shared.shape != (batch, beams, beams)):
+            raise A.MsaError("reorder: parent [batch, beams], length [batch] and shared [batch, beams, beams] expected")
+        for t in (slot, parent, length, shared):
+            if t is not None and (t.dtype != torch.int32 or t.device != self.last_token.device or not t.is_contiguous()):
+                raise A.MsaError("reorder: contiguous int32 tables on the cache's device expected")
+        slot_out, shared_out = torch.empty_like(slot), None if shared is None else torch.empty_like(shared)
+        if batch:
+            parts = self._state_parts()
+            with A.on_device(slot.device):
+                work = torch.empty(A.lib().msa_lm_reorder_workspace(batch, beams, parts.shape[0]), dtype=torch.uint8, device=slot.device)
+                A.call("msa_lm_reorder", A.ptr(slot), A.ptr(parent), A.ptr(length), A.ptr(shared), batch, beams, self.n_slots, A.ptr(parts),
+                       parts.shape[0], A.ptr(slot_out), A.ptr(shared_out), A.ptr(work), A.stream_ptr(slot.device))
+        return slot_out, shared_out
 
     def state_bytes(self) -> int:
         return sum(t.numel() * t.element_size() for d in (self.ring, self.state, self.conv, self.shift) for t in d.values())

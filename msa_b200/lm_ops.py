@@ -159,6 +159,46 @@ def argmax(logits: torch.Tensor) -> torch.Tensor:
     return out
 
 
+BEAM_MAX, BEAM_MAX_K = 32, 64        # kBeamMax, kBeamMaxK
+
+
+def beam_topk(logits: torch.Tensor, scores: torch.Tensor, k: int, stop: Optional[torch.Tensor] = None):
+    """The ``k`` best continuations of every question's beams: ``(score fp32, beam, token)``, each ``[batch, k]`` in descending order.
+
+    ``scores`` fp32 ``[batch, beams]``; row ``q * beams + b`` of ``logits`` (fp32 or bf16 ``[batch * beams, vocab]``, rows with a
+    contiguous last axis) belongs to beam b of question q.  Continuation (b, t) has the score ``scores[q, b] + log_softmax(row)[t]``, ordered
+    in 64 bits; equals go to the lower beam, then to the larger logit, then to the lower token.  Logits of -inf are no continuations, nor is anything of a beam whose score is not
+    finite or whose row holds a NaN or +inf; places left over hold ``(-inf, -1, -1)``.
+
+    With ``stop`` (int32 token ids, may be empty) three more, ``[batch, beams]``: the first ``beams`` of the k whose token is not
+    among them, which are the next beams (``k >= beams * (1 + len(stop))`` always finds that many, where there are that many)."""
+    A.need_cuda(logits, scores, stop)
+    if logits.dim() != 2 or scores.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16) or scores.dtype != torch.float32:
+        raise A.MsaError("beam_topk: fp32 or bf16 logits [batch * beams, vocab] and fp32 scores [batch, beams] expected")
+    (batch, beams), (rows, vocab) = scores.shape, logits.shape
+    if rows != batch * beams or not 1 <= beams <= BEAM_MAX or vocab < 1:
+        raise A.MsaError(f"beam_topk: {rows} rows of {vocab} logits for {batch} questions of {beams} beams (1 to {BEAM_MAX})")
+    if not 1 <= k <= min(BEAM_MAX_K, beams * vocab):
+        raise A.MsaError(f"beam_topk: k = {k} of {beams * vocab} continuations (1 to {BEAM_MAX_K})")
+    if logits.stride(1) != 1 and vocab > 1:
+        raise A.MsaError("rows with a contiguous last axis expected")
+    dev = logits.device
+    if scores.device != dev or not scores.is_contiguous():
+        raise A.MsaError("beam_topk: contiguous scores on the logits' device expected")
+    if stop is not None and (stop.device != dev or stop.dtype != torch.int32 or stop.dim() != 1 or not stop.is_contiguous()):
+        raise A.MsaError("beam_topk: stop tokens must be a contiguous int32 vector on the logits' device")
+    new = lambda n, dt: torch.empty((batch, n), dtype=dt, device=dev)
+    out = [new(k, torch.float32), new(k, torch.int32), new(k, torch.int32)]
+    if stop is not None:
+        out += [new(beams, torch.float32), new(beams, torch.int32), new(beams, torch.int32)]
+    if batch:
+        with A.on_device(dev):
+            work = torch.empty(A.lib().msa_lm_beam_topk_workspace(batch, beams, vocab, k), dtype=torch.uint8, device=dev)
+            A.call("msa_lm_beam_topk", A.ptr(logits), logits.stride(0), A.dtype_code(logits.dtype), A.ptr(scores), batch, beams, vocab, k, A.ptr(stop),
+                   0 if stop is None else stop.shape[0], A.ptr(work), *(A.ptr(t) for t in out), *([0] * (6 - len(out))), A.stream_ptr(dev))
+    return tuple(out)
+
+
 def token_shift(h, mu, step, shift):
     """``[mixes, n, width]``: every row of ``h`` mixed with its sequence's previous one (``shift`` keeps the last rows)."""
     A.need_cuda(h, mu)
