@@ -13,27 +13,58 @@ namespace msa {
 constexpr int kBeamMax = 32;             // beams of a question: a warp
 constexpr int kBeamMaxK = 64;
 constexpr int kBcThreads = 256, kBcWarps = kBcThreads / 32, kBcPer = 16, kBcTile = kBcThreads * kBcPer;
-constexpr int kBcCap = 1024;             // candidates of a tile that wait to be ranked
+constexpr int kBcCap = 1024;             // entries of a part that wait to be ranked
+constexpr int kBjThreads = 512, kBjWarps = kBjThreads / 32;
 
-struct BeamRank { uint32_t key; int32_t idx; };      // float_to_key of the logit; equals: the lower index is better
-__device__ __forceinline__ bool better(uint32_t ka, int ia, uint32_t kb, int ib) { return ka > kb || (ka == kb && ia < ib); }
-constexpr uint32_t kNoKey = 0x007fffffu;              // float_to_key(-inf): no candidate at or below it (NaN never enters)
+// A logit and its token as one number: the larger logit is better, of equals the lower token.  0: none; NaN and -inf never enter.
+typedef unsigned long long Rank;
+constexpr uint32_t kNoKey = 0x007fffffu;              // float_to_key(-inf)
+__device__ __forceinline__ Rank rank_of(float x, int idx) { return (Rank)float_to_key(x + 0.f) << 32 | (uint32_t)~idx; }   // -0 is 0
+__device__ __forceinline__ uint32_t rank_key(Rank r) { return (uint32_t)(r >> 32); }
+__device__ __forceinline__ int rank_idx(Rank r) { return (int)~(uint32_t)r; }
 
-// A row's part: sum = sum exp(x - ref) over its logits (NaN: a logit was NaN or +inf), and its best logits in order.
-struct BeamPart { double ref, sum; };
+// A row's part: the sum of e^x over its logits as sum * 2^n * e^base (NaN: a logit was NaN or +inf).
+struct BeamPart { double sum; int32_t n; float base; };
 
-// The `want`-th best of a warp's lanes' (key, idx) pairs; key 0 where there are fewer candidates.
-__device__ __forceinline__ BeamRank warp_nth(uint32_t key, int idx, int want) {
-  BeamRank r{0u, 0x7fffffff};
-  for (int i = 0; i < want; ++i) {
-    r.key = __reduce_max_sync(0xffffffffu, key);
-    if (r.key <= kNoKey) return {0u, 0x7fffffff};
-    r.idx = __reduce_min_sync(0xffffffffu, key == r.key ? idx : 0x7fffffff);
-    if (key == r.key && idx == r.idx) key = 0u;
+// p += v.
+__device__ __forceinline__ double pow2(float e) { return e < -1000.f ? 0.0 : __longlong_as_double((long long)((int)e + 1023) << 52); }   // whole e <= 0
+__device__ __forceinline__ void join_sums(BeamPart& p, const BeamPart& v) {
+  if (v.sum == 0.0) return;
+  if (p.sum == 0.0) { p = v; return; }
+  if (p.base == 0.f && v.base == 0.f) {
+    const int n = max(p.n, v.n);
+    p.sum = p.sum * pow2((float)(p.n - n)) + v.sum * pow2((float)(v.n - n));
+    p.n = n;
+    return;
   }
-  return r;
+  const double rp = (double)p.base + p.n * 0.6931471805599453, rv = (double)v.base + v.n * 0.6931471805599453;
+  if (rp >= rv) { p.sum += v.sum * exp(rv - rp); return; }
+  const double mine = p.sum * exp(rp - rv);
+  p = v;
+  p.sum += mine;
 }
 
+__device__ __forceinline__ BeamPart other_part(const BeamPart& p, int o) {
+  return {__shfl_xor_sync(0xffffffffu, p.sum, o), __shfl_xor_sync(0xffffffffu, p.n, o), __shfl_xor_sync(0xffffffffu, p.base, o)};
+}
+
+// The `want`-th best of a warp's lanes, each with one entry; 0 where there are fewer.
+__device__ __forceinline__ Rank warp_nth(Rank mine, int want) {
+  uint32_t key = 0u, low = 0u;
+  for (int i = 0; i < want; ++i) {
+    key = __reduce_max_sync(0xffffffffu, rank_key(mine));
+    if (key <= kNoKey) return 0ull;
+    low = __reduce_max_sync(0xffffffffu, rank_key(mine) == key ? (uint32_t)mine : 0u);
+    if (mine == ((Rank)key << 32 | low)) mine = 0ull;
+  }
+  return (Rank)key << 32 | low;
+}
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 __device__ __forceinline__ float ex2_part(float f) {      // |f| <= 1/2
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(f));
@@ -41,155 +72,229 @@ __device__ __forceinline__ float ex2_part(float f) {      // |f| <= 1/2
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kBcThreads)
+__device__ __forceinline__ void load_tile(const T* x_row, int t, int v1, float (&x)[kBcPer]) {
+  if (t + kBcTile <= v1) {
+#pragma unroll
+    for (int j = 0; j < kBcPer; ++j) x[j] = to_f(x_row[t + j * kBcThreads + (int)threadIdx.x]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kBcPer; ++j) {
+      const int i = t + j * kBcThreads + (int)threadIdx.x;
+      x[j] = i < v1 ? to_f(x_row[i]) : -INFINITY;
+    }
+  }
+}
+
+struct BeamScratch { Rank list[2][kBeamMaxK], fresh[kBcCap], post[kBcWarps]; int count; };
+
+// Entries 0 .. n-1 of s.fresh join the `have` of s.list[cur], which are in order: each one's place is the number of better ones.
+__device__ __forceinline__ void rank_entries(BeamScratch& s, int n, int k, int& have, int& cur) {
+  for (int i = threadIdx.x; i < have + n; i += kBcThreads) {
+    const Rank mine = i < have ? s.list[cur][i] : s.fresh[i - have];
+    int place = i < have ? i : 0;
+    if (i >= have) for (int o = 0; o < have; ++o) place += s.list[cur][o] > mine;
+#pragma unroll 4
+    for (int o = 0; o < n; ++o) place += s.fresh[o] > mine;
+    if (place < k) s.list[cur ^ 1][place] = mine;
+  }
+  cur ^= 1;
+  have = min(k, have + n);
+  __syncthreads();
+}
+
+// The k best of a part whatever its order, tile by tile, where too many entries passed the bound on the way (rows that rise towards their
+// end, masks that leave a warp without logits): 64 beams over 12,345 sorted logits take 1.7 times as long as unsorted ones.
+template <typename T>
+__device__ __noinline__ int ordered_best(const T* x_row, int v0, int v1, int k, BeamScratch& s) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, want = (k + kBcWarps - 1) / kBcWarps;
+  int have = 0, cur = 0;
+  Rank kth = 0ull;                                          // what a newcomer has to beat
+  for (int t = v0; t < v1; t += kBcTile) {
+    float x[kBcPer];
+    load_tile(x_row, t, v1, x);
+    Rank best = 0ull;
+#pragma unroll
+    for (int j = 0; j < kBcPer; ++j) {
+      const Rank e = rank_of(x[j], t + j * kBcThreads + (int)threadIdx.x);
+      if (x[j] > -INFINITY && e > best) best = e;
+    }
+    const Rank post = warp_nth(best, want);
+    __syncthreads();
+    if (lane == 0) s.post[warp] = post;
+    if (threadIdx.x == 0) s.count = 0;
+    __syncthreads();
+    Rank bound = s.post[0];
+#pragma unroll
+    for (int w = 1; w < kBcWarps; ++w) bound = min(bound, s.post[w]);
+#pragma unroll
+    for (int j = 0; j < kBcPer; ++j) {
+      const Rank e = rank_of(x[j], t + j * kBcThreads + (int)threadIdx.x);
+      if (x[j] > -INFINITY && e > kth && e >= bound) {
+        const int at = atomicAdd(&s.count, 1);
+        if (at < kBcCap) s.fresh[at] = e;
+      }
+    }
+    __syncthreads();
+    int n = s.count;
+    if (n > kBcCap) {                                       // the bound says nothing: one at a time, each the best behind the one before
+      Rank last = ~0ull;
+      for (n = 0; n < k; ++n) {
+        best = 0ull;
+#pragma unroll
+        for (int j = 0; j < kBcPer; ++j) {
+          const Rank e = rank_of(x[j], t + j * kBcThreads + (int)threadIdx.x);
+          if (x[j] > -INFINITY && e > kth && e < last && e > best) best = e;
+        }
+        best = warp_nth(best, 1);
+        __syncthreads();
+        if (lane == 0) s.post[warp] = best;
+        __syncthreads();
+        last = s.post[0];
+#pragma unroll
+        for (int w = 1; w < kBcWarps; ++w) last = max(last, s.post[w]);
+        if (last == 0ull) break;
+        if (threadIdx.x == 0) s.fresh[n] = last;
+      }
+      __syncthreads();
+    }
+    rank_entries(s, n, k, have, cur);
+    if (have == k) kth = s.list[cur][k - 1];
+  }
+  if (cur) {
+    for (int i = threadIdx.x; i < have; i += kBcThreads) s.list[0][i] = s.list[1][i];
+    __syncthreads();
+  }
+  return have;
+}
+
+// One block per part of a row.  Its warps walk the part's tiles without waiting for one another: each keeps its lanes' best logits and
+// publishes the want-th of them, want = ceil(k / 8), so that the least of the eight is a bound that k logits reach; what reaches it is
+// set aside, some 2.5 k (1 + log tiles) entries, and ranked at the end.  The next tile's loads are in flight meanwhile.
+template <typename T>
+__global__ void __launch_bounds__(kBcThreads, 3)
 beam_rows_kernel(const T* __restrict__ logits, long long stride, const float* __restrict__ scores, int vocab, int splits, int tiles_per_split, int k,
-                 BeamPart* __restrict__ parts, BeamRank* __restrict__ best) {
-  __shared__ BeamRank s_list[2][kBeamMaxK], s_new[kBcCap], s_thr[kBcWarps];
-  __shared__ uint32_t s_max[kBcWarps];
-  __shared__ int s_count;
+                 BeamPart* __restrict__ parts, Rank* __restrict__ best) {
+  __shared__ BeamScratch s;
   __shared__ double s_sum[kBcWarps];
+  __shared__ int s_n[kBcWarps];
+  __shared__ float s_base[kBcWarps];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const long long row = blockIdx.x / splits, part = blockIdx.x;
-  const int t0 = (int)(blockIdx.x % splits) * tiles_per_split, v0 = t0 * kBcTile, v1 = (int)min((long long)vocab, (long long)v0 + (long long)tiles_per_split * kBcTile);
-  const float score = scores[row];
-  BeamRank* out = best + part * k;
-  if (!(fabsf(score) < INFINITY) || v0 >= vocab) {           // a beam without a score offers nothing
-    if (tid < k) out[tid] = {0u, 0x7fffffff};
-    if (tid == 0) parts[part] = {0.0, 0.0};
+  const int v0 = (int)(blockIdx.x % splits) * tiles_per_split * kBcTile, v1 = (int)min((long long)vocab, (long long)v0 + (long long)tiles_per_split * kBcTile);
+  Rank* out = best + part * k;
+  if (!(fabsf(scores[row]) < INFINITY)) {                    // a beam without a score offers nothing
+    if (tid < k) out[tid] = 0ull;
+    if (tid == 0) parts[part] = {0.0, 0, 0.f};
     return;
   }
   const T* x_row = logits + row * stride;
   const int want = (k + kBcWarps - 1) / kBcWarps;
-  int have = 0, cur = 0;                                    // entries of s_list[cur], in order
-  BeamRank kth{kNoKey, 0x7fffffff};                         // what a newcomer has to beat
-  uint32_t top = 0u;                                        // key of the largest logit so far
-  float base = 0.f, big_n = 0.f;                            // the sum's reference: base + big_n * ln 2
-  double ref = 0.0, sum = 0.0;
+  float x[kBcPer];
+  load_tile(x_row, v0, v1, x);
+  if (tid == 0) s.count = 0;
+  float mine = -INFINITY;                                   // this lane's best, its token, and the warp's best
+  int mine_at = 0;
+  uint32_t top = 0u;
+  float base = 0.f, big_n = 0.f;                            // the warp's reference
+  double sum = 0.0;
   bool nan = false;
-  if (tid == 0) s_count = 0;
   for (int t = v0; t < v1; t += kBcTile) {
-    float x[kBcPer];
+    float nx[kBcPer];
+    if (t + kBcTile < v1) load_tile(x_row, t + kBcTile, v1, nx);
+    float m = x[0], m2 = x[1];
 #pragma unroll
-    for (int j = 0; j < kBcPer; ++j) {
-      const int i = t + j * kBcThreads + tid;
-      x[j] = i < v1 ? to_f(x_row[i]) : -INFINITY;
+    for (int j = 2; j < kBcPer; j += 2) { m = max_nan(m, x[j]); m2 = max_nan(m2, x[j + 1]); }
+    m = max_nan(m, m2);
+    if (m != m) {                                           // the maximum that passes over NaN
+      nan = true;
+      m = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < kBcPer; ++j) m = fmaxf(m, x[j]);
     }
-    float m = -INFINITY;
+    if (__any_sync(0xffffffffu, m > mine)) {
+      if (m > mine) {
+        mine = m;
 #pragma unroll
-    for (int j = 0; j < kBcPer; ++j) { m = fmaxf(m, x[j]); nan |= x[j] != x[j]; }
-    const uint32_t key = float_to_key(m);
-    // A lower bound of the tile's k best: each of the eight warps has `want` lanes whose best is at least the least of the warps'
-    // want-th best.  It is a pair with an index, so that equal logits do not all pass.
-    const uint32_t w_max = __reduce_max_sync(0xffffffffu, key);
-    BeamRank thr{0u, 0x7fffffff};
-    if (w_max > kth.key) {
-      int at = 0;
-#pragma unroll
-      for (int j = kBcPer - 1; j >= 0; --j) if (x[j] == m) at = j;
-      thr = warp_nth(key, t + at * kBcThreads + tid, want);
+        for (int j = kBcPer - 1; j >= 0; --j) if (x[j] == m) mine_at = t + j * kBcThreads + tid;
+      }
+      const Rank post = warp_nth(mine > -INFINITY ? rank_of(mine, mine_at) : 0ull, want);
+      if (lane == 0) *(volatile Rank*)&s.post[warp] = post;
+      const uint32_t t_max = __reduce_max_sync(0xffffffffu, float_to_key(m));
+      if (t_max > top) {
+        // The sum is kept relative to a power of two, which moves no bit of a term (and to e^base for logits beyond 1e6).
+        const float mx = key_to_float(t_max), new_base = fabsf(mx) < 1e6f ? 0.f : mx, new_n = rintf((mx - new_base) * 1.44269504f);
+        if (sum != 0.0) sum *= new_base == 0.f && base == 0.f ? pow2(big_n - new_n) : exp(((double)base - new_base) + ((double)big_n - new_n) * 0.6931471805599453);
+        top = t_max; base = new_base; big_n = new_n;
+      }
+    } else if (t == v0 && lane == 0) {
+      s.post[warp] = 0ull;                                  // nothing but -inf
     }
-    if (lane == 0) { s_max[warp] = w_max; s_thr[warp] = thr; }
-    __syncthreads();
-    uint32_t t_max = s_max[0];
-    thr = s_thr[0];
+    if (t == v0) __syncthreads();                           // later a bound that is behind lets a few more pass
+    Rank bound = *(volatile Rank*)&s.post[0];
 #pragma unroll
-    for (int w = 1; w < kBcWarps; ++w) {
-      t_max = max(t_max, s_max[w]);
-      if (better(thr.key, thr.idx, s_thr[w].key, s_thr[w].idx)) thr = s_thr[w];
-    }
-    if (t_max > top) {
-      top = t_max;
-      // The sum is kept relative to 2^big_n (times e^base for logits beyond 1e6): a power of two moves no bit of a term.
-      const float mx = key_to_float(top);
-      const float new_base = fabsf(mx) < 1e6f ? 0.f : mx, new_n = rintf((mx - new_base) * 1.44269504f);
-      const double new_ref = (double)new_base + (double)new_n * 0.6931471805599453;
-      if (sum != 0.0) sum *= exp(ref - new_ref);
-      base = new_base; big_n = new_n; ref = new_ref;
-    }
-    if (key > kth.key) {
-      if (t_max > kth.key) {
+    for (int w = 1; w < kBcWarps; ++w) bound = min(bound, *(volatile Rank*)&s.post[w]);
+    const float least = rank_key(bound) > kNoKey ? key_to_float(rank_key(bound)) : -INFINITY;
+    if (m >= least) {
 #pragma unroll
-        for (int j = 0; j < kBcPer; ++j) {
-          const uint32_t e = float_to_key(x[j]);
-          const int i = t + j * kBcThreads + tid;
-          if (x[j] == x[j] && e > kth.key && e >= thr.key && (e > thr.key || i <= thr.idx)) {
-            const int at = atomicAdd(&s_count, 1);
-            if (at < kBcCap) s_new[at] = {e, i};
+      for (int j = 0; j < kBcPer; ++j)
+        if (x[j] >= least) {
+          const Rank e = rank_of(x[j], t + j * kBcThreads + tid);
+          if (e >= bound && x[j] > -INFINITY) {
+            const int at = atomicAdd(&s.count, 1);
+            if (at < kBcCap) s.fresh[at] = e;
           }
         }
-      }
     }
     if (top > kNoKey) {
-      // exp(x - base) / 2^big_n: the whole part of the exponent by integer arithmetic, the fraction (exact to 2^-25) by ex2.
-      const float floor_x = key_to_float(top) - 80.f;         // below e^-80 of the largest: nothing in the sum's 53 bits
+      // e^x / 2^big_n: the exponent's whole part by integer arithmetic, the fraction (exact to 2^-25) by ex2.
+      const float floor_x = key_to_float(top) - 80.f, magic = 12582912.f - big_n;
       float a = 0.f, b = 0.f;
+      if (base == 0.f) {
 #pragma unroll
-      for (int j = 0; j < kBcPer; ++j) {
-        const float y = fmaxf(x[j], floor_x) - base;
-        const float r = fmaf(y, 1.44269504f, 12582912.f), n = r - 12582912.f;
-        const float f = fmaf(y, 1.92596299e-8f, fmaf(y, 1.44269502f, -n));
-        const float e = x[j] >= floor_x ? __int_as_float(__float_as_int(ex2_part(f)) + ((int)(n - big_n) << 23)) : 0.f;
-        if (j & 1) b += e; else a += e;
+        for (int j = 0; j < kBcPer; ++j) {
+          const float y = fmaxf(x[j], floor_x);             // e^-80 of the largest is nothing in the sum's 53 bits, and -inf may count as that
+          const float r = fmaf(y, 1.44269504f, magic), f = fmaf(y, 1.92596299e-8f, fmaf(y, 1.44269502f, magic - r));
+          const float e = __int_as_float(__float_as_int(ex2_part(f)) + (__float_as_int(r) << 23));
+          if (j & 1) b += e; else a += e;
+        }
+      } else {                                              // big_n is 0
+#pragma unroll
+        for (int j = 0; j < kBcPer; ++j) a += x[j] >= floor_x ? expf(x[j] - base) : 0.f;
       }
       sum += (double)(a + b);
     }
-    __syncthreads();
-    int n_new = s_count;
-    if (n_new > kBcCap) {
-      // Hardly ever: the warps' bests say little about the rest (a tile in which one warp's logits are all masked).  The k best
-      // one at a time, each the best behind the one before.
-      BeamRank last{0xffffffffu, -1};
-      n_new = 0;
-      while (n_new < k) {
-        BeamRank mine{0u, 0x7fffffff};
 #pragma unroll
-        for (int j = 0; j < kBcPer; ++j) {
-          const uint32_t e = float_to_key(x[j]);
-          const int i = t + j * kBcThreads + tid;
-          if (x[j] == x[j] && e > kth.key && better(last.key, last.idx, e, i) && better(e, i, mine.key, mine.idx)) mine = {e, i};
-        }
-        mine = warp_nth(mine.key, mine.idx, 1);
-        if (lane == 0) s_thr[warp] = mine;
-        __syncthreads();
-        mine = s_thr[0];
-#pragma unroll
-        for (int w = 1; w < kBcWarps; ++w) if (better(s_thr[w].key, s_thr[w].idx, mine.key, mine.idx)) mine = s_thr[w];
-        __syncthreads();
-        if (mine.key == 0u) break;
-        if (tid == 0) s_new[n_new] = mine;
-        last = mine;
-        ++n_new;
-      }
-      __syncthreads();
-    }
-    if (n_new > 0) {
-      // Each entry's place is the number of better ones.
-      const int all = have + n_new;
-      for (int i = tid; i < all; i += kBcThreads) {
-        const BeamRank mine = i < have ? s_list[cur][i] : s_new[i - have];
-        int place = i < have ? i : 0;                         // the old ones are in order
-        if (i >= have) for (int o = 0; o < have; ++o) place += better(s_list[cur][o].key, s_list[cur][o].idx, mine.key, mine.idx);
-        for (int o = 0; o < n_new; ++o) place += better(s_new[o].key, s_new[o].idx, mine.key, mine.idx);
-        if (place < k) s_list[cur ^ 1][place] = mine;
-      }
-      cur ^= 1;
-      have = min(k, all);
-      __syncthreads();
-      if (have == k) kth = s_list[cur][k - 1];
-      if (tid == 0) s_count = 0;
-    }
+    for (int j = 0; j < kBcPer; ++j) x[j] = nx[j];
   }
-  if (tid < k) out[tid] = tid < have ? s_list[cur][tid] : BeamRank{0u, 0x7fffffff};
-  nan = nan || top >= float_to_key(INFINITY);
-  double s = nan ? __longlong_as_double(0x7ff8000000000000ll) : sum;
+  if (nan || top >= float_to_key(INFINITY)) sum = __longlong_as_double(0x7ff8000000000000ll);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if (lane == 0) s_sum[warp] = s;
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) { s_sum[warp] = sum; s_n[warp] = (int)big_n; s_base[warp] = base; }
   __syncthreads();
-  if (tid == 0) {
-    s = s_sum[0];
-    for (int w = 1; w < kBcWarps; ++w) s += s_sum[w];
-    parts[part] = {ref, s};
+  int n = s.count, have = 0, cur = 0;
+  if (n > kBcCap) {
+    have = ordered_best(x_row, v0, v1, k, s);
+  } else {
+    // What reaches the bound of all tiles is what remains: every thread holds up to four of the entries meanwhile.
+    Rank bound = s.post[0], keep[kBcCap / kBcThreads];
+#pragma unroll
+    for (int w = 1; w < kBcWarps; ++w) bound = min(bound, s.post[w]);
+#pragma unroll
+    for (int i = 0; i < kBcCap / kBcThreads; ++i) keep[i] = i * kBcThreads + tid < n ? s.fresh[i * kBcThreads + tid] : 0ull;
+    __syncthreads();
+    if (tid == 0) s.count = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kBcCap / kBcThreads; ++i) if (keep[i] != 0ull && keep[i] >= bound) s.fresh[atomicAdd(&s.count, 1)] = keep[i];
+    __syncthreads();
+    rank_entries(s, s.count, k, have, cur);
+  }
+  if (tid < k) out[tid] = tid < have ? s.list[cur][tid] : 0ull;
+  if (warp == kBcWarps - 1) {
+    BeamPart p = {s_sum[lane % kBcWarps], s_n[lane % kBcWarps], s_base[lane % kBcWarps]};
+#pragma unroll
+    for (int o = 1; o < kBcWarps; o <<= 1) join_sums(p, other_part(p, o));
+    if (lane == 0) parts[part] = p;
   }
 }
 
@@ -226,91 +331,90 @@ __device__ __forceinline__ BeamScore warp_best(BeamScore v, const BeamOrder& bet
 
 struct BeamChoiceOut { float* score; int32_t *beam, *token; float* live_score; int32_t *live_beam, *live_token; };
 
-// One block per question.
-__global__ void __launch_bounds__(kBcThreads)
-beam_join_kernel(const BeamPart* __restrict__ parts, const BeamRank* __restrict__ best, const float* __restrict__ scores, int beams, int vocab,
-                 int splits, int k, const int32_t* __restrict__ stop, int n_stop, const BeamChoiceOut out) {
+// One block per question.  Scores are 64-bit; a bound from below, in 32 bits rounded down, leaves a few times k candidates to rank.
+__global__ void __launch_bounds__(kBjThreads)
+beam_join_kernel(const BeamPart* parts, const Rank* best, const float* scores, int beams, int vocab, int splits, int k, const int32_t* stop, int n_stop,
+                 const BeamChoiceOut out) {
+  grid_dependency_wait();
+  __shared__ BeamPart s_part[kBeamMax];
   __shared__ double s_lse[kBeamMax], s_score[kBeamMax];
-  __shared__ BeamScore s_new[kBcCap], s_thr[kBcWarps], s_done[kBeamMaxK];
+  __shared__ BeamScore s_new[kBcCap], s_one[kBjWarps], s_done[kBeamMaxK];
+  __shared__ uint32_t s_post[kBjWarps];
   __shared__ int s_count;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const long long q = blockIdx.x;
   const BeamOrder better{vocab};
   if (tid == 0) s_count = 0;
-  for (int b = warp; b < beams; b += kBcWarps) {
-    const BeamPart* p = parts + (q * beams + b) * splits;
-    double m = -INFINITY, s = 0.0;
-    for (int i = lane; i < splits; i += 32) {
-      const BeamPart v = p[i];
-      if (v.sum != 0.0) {                                     // NaN too
-        const double mx = fmax(m, v.ref);
-        s = s * exp(m - mx) + v.sum * exp(v.ref - mx);
-        m = mx;
-      }
-    }
+  for (int b = warp; b < beams; b += kBjWarps) {
+    BeamPart p = {0.0, 0, 0.f};
+    for (int i = lane; i < splits; i += 32) join_sums(p, parts[(q * beams + b) * splits + i]);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const double om = __shfl_xor_sync(0xffffffffu, m, o), os = __shfl_xor_sync(0xffffffffu, s, o), mx = fmax(m, om);
-      if (mx > -INFINITY) s = s * exp(m - mx) + os * exp(om - mx);
-      m = mx;
-    }
-    if (lane == 0) { s_lse[b] = m + log(s); s_score[b] = (double)scores[q * beams + b]; }    // nothing summed, or NaN: no candidates below
+    for (int o = 16; o > 0; o >>= 1) join_sums(p, other_part(p, o));
+    if (lane == 0) s_part[b] = p;
   }
   __syncthreads();
-  const int per_row = splits * k, n = beams * per_row;
+  if (tid < beams) {                                          // nothing summed, or NaN: no candidates below
+    const BeamPart p = s_part[tid];
+    s_lse[tid] = ((double)p.base + (double)p.n * 0.6931471805599453) + log(p.sum);
+    s_score[tid] = (double)scores[q * beams + tid];
+  }
+  __syncthreads();
+  // Candidates are taken the parts' best ones first, so that every warp sees some of those.
+  const int lists = beams * splits, n = lists * k;
+  const Rank* ranks = best + q * n;
   auto candidate = [&](int c) -> BeamScore {
-    const int b = c / per_row;
-    const BeamRank r = best[(q * beams + b) * per_row + (c - b * per_row)];
-    if (r.key <= kNoKey) return kNoScore;
-    const double v = s_score[b] + ((double)key_to_float(r.key) - s_lse[b]);
-    return v > -INFINITY && v < INFINITY ? BeamScore{score_key(v), b * vocab + r.idx, r.key} : kNoScore;
+    const int place = c / lists, list = c - place * lists, b = list / splits;
+    const Rank r = ranks[list * k + place];
+    if (r == 0ull) return kNoScore;
+    const double v = s_score[b] + ((double)key_to_float(rank_key(r)) - s_lse[b]);
+    return v > -INFINITY && v < INFINITY ? BeamScore{score_key(v), b * vocab + rank_idx(r), rank_key(r)} : kNoScore;
   };
-  BeamScore mine = kNoScore;
-  for (int c = tid; c < n; c += kBcThreads) {
-    const BeamScore v = candidate(c);
-    if (better(v, mine)) mine = v;
+  unsigned long long top = 0ull;
+  for (int c = tid; c < n; c += kBjThreads) top = max(top, candidate(c).key);
+  uint32_t key = top ? float_to_key(__double2float_rd(key_score(top))) : 0u, post = 0u;
+  const int warps = min(kBjWarps, (n + 31) / 32);               // those with candidates: each has `want` that reach the bound
+  for (int i = 0, want = (k + warps - 1) / warps; i < want; ++i) {
+    post = __reduce_max_sync(0xffffffffu, key);
+    const unsigned who = __ballot_sync(0xffffffffu, key == post);
+    if (lane == __ffs(who) - 1) key = 0u;
   }
-  // As for a tile: the least of the warps' want-th best lanes bounds the k best from below.
-  BeamScore thr = kNoScore;
-  for (int i = 0, want = (k + kBcWarps - 1) / kBcWarps; i < want; ++i) {
-    thr = warp_best(mine, better);
-    if (mine.key == thr.key && mine.at == thr.at) mine = kNoScore;
-  }
-  if (lane == 0) s_thr[warp] = thr;
+  if (lane == 0) s_post[warp] = post;
   __syncthreads();
-  thr = s_thr[0];
-  for (int w = 1; w < kBcWarps; ++w) if (better(thr, s_thr[w])) thr = s_thr[w];
-  for (int c = tid; c < n; c += kBcThreads) {
+  uint32_t bound = s_post[0];
+  for (int w = 1; w < warps; ++w) bound = min(bound, s_post[w]);
+  const unsigned long long least = bound ? score_key((double)key_to_float(bound)) : 1ull;
+  for (int c = tid; c < n; c += kBjThreads) {
     const BeamScore v = candidate(c);
-    if (v.key && !better(thr, v)) {
+    if (v.key >= least) {
       const int at = atomicAdd(&s_count, 1);
       if (at < kBcCap) s_new[at] = v;
     }
   }
   __syncthreads();
   int have = s_count;
-  if (have > kBcCap) {                                        // hardly ever: one at a time
+  if (have > kBcCap) {                                        // equal scores by the hundred: one at a time
     BeamScore last{~0ull, -1, ~0u};
     for (have = 0; have < k; ++have) {
-      mine = kNoScore;
-      for (int c = tid; c < n; c += kBcThreads) {
+      BeamScore mine = kNoScore;
+      for (int c = tid; c < n; c += kBjThreads) {
         const BeamScore v = candidate(c);
         if (v.key && better(last, v) && better(v, mine)) mine = v;
       }
       mine = warp_best(mine, better);
-      if (lane == 0) s_thr[warp] = mine;
+      if (lane == 0) s_one[warp] = mine;
       __syncthreads();
-      mine = s_thr[0];
-      for (int w = 1; w < kBcWarps; ++w) if (better(s_thr[w], mine)) mine = s_thr[w];
+      mine = s_one[0];
+      for (int w = 1; w < kBjWarps; ++w) if (better(s_one[w], mine)) mine = s_one[w];
       __syncthreads();
       if (!mine.key) break;
       if (tid == 0) s_done[have] = mine;
       last = mine;
     }
   } else {
-    for (int i = tid; i < have; i += kBcThreads) {
+    for (int i = tid; i < have; i += kBjThreads) {
       const BeamScore v = s_new[i];
       int place = 0;
+#pragma unroll 4
       for (int o = 0; o < have; ++o) place += better(s_new[o], v);
       if (place < k) s_done[place] = v;
     }
@@ -498,7 +602,7 @@ reorder_copy_kernel(const msa_lm_state_part* part, int n_part, const ReorderCopy
 
 template <typename T>
 void launch_beam_rows(const void* logits, int64_t stride, const float* scores, int64_t rows, int vocab, int splits, int tiles_per_split, int k,
-                      BeamPart* parts, BeamRank* best, cudaStream_t st) {
+                      BeamPart* parts, Rank* best, cudaStream_t st) {
   beam_rows_kernel<T><<<(unsigned)(rows * splits), kBcThreads, 0, st>>>((const T*)logits, stride, scores, vocab, splits, tiles_per_split, k, parts, best);
 }
 
@@ -519,7 +623,7 @@ extern "C" int64_t msa_lm_beam_topk_workspace(int32_t batch, int32_t beams, int3
   if (batch <= 0 || beams <= 0 || vocab <= 0 || k <= 0) return 0;
   int per = 0;
   const int64_t parts = (int64_t)batch * beams * beam_splits((int64_t)batch * beams, vocab, &per);
-  return parts * ((int64_t)sizeof(BeamPart) + (int64_t)k * (int64_t)sizeof(BeamRank));
+  return parts * ((int64_t)sizeof(BeamPart) + (int64_t)k * (int64_t)sizeof(Rank));
 }
 
 extern "C" int msa_lm_beam_topk(const void* logits, int64_t stride, int32_t dtype, const float* scores, int32_t batch, int32_t beams, int32_t vocab,
@@ -538,12 +642,13 @@ extern "C" int msa_lm_beam_topk(const void* logits, int64_t stride, int32_t dtyp
   const int splits = beam_splits(rows, vocab, &per);
   MSA_REQUIRE(rows * splits < (1ll << 31), "beam_topk: too many rows");
   BeamPart* parts = (BeamPart*)workspace;
-  BeamRank* best = (BeamRank*)(parts + rows * splits);
+  Rank* best = (Rank*)(parts + rows * splits);
   cudaStream_t st = (cudaStream_t)stream;
   MSA_LM_DISPATCH(dtype, { launch_beam_rows<T>(logits, stride, scores, rows, vocab, splits, per, k, parts, best, st); });
   MSA_LAUNCH_OK("beam_rows_kernel");
   const BeamChoiceOut out{score, beam, token, live_score, live_beam, live_token};
-  beam_join_kernel<<<(unsigned)batch, kBcThreads, 0, st>>>(parts, best, scores, beams, vocab, splits, k, stop, n_stop, out);
+  MSA_CUDA_OK(launch_kernel_pdl(beam_join_kernel, dim3((unsigned)batch), dim3(kBjThreads), 0, st, true, parts, best, scores, beams, vocab, splits, k, stop,
+                                n_stop, out));
   MSA_LAUNCH_OK("beam_join_kernel");
   return MSA_OK;
 }
