@@ -7,27 +7,23 @@
 // Reordering.  New beam j continues beam parent[j].  Its first child keeps a beam's slot, the others take slots that nobody
 // continues: sources and destinations never meet, and no second buffer is needed.  Bound by the copied bytes, read and written once.
 #include "lm_common.cuh"
+#include "tc_attn_common.cuh"
 
 namespace msa {
 
 constexpr int kBeamMax = 32;             // beams of a question: a warp
 constexpr int kBeamMaxK = 64;
-constexpr int kBcThreads = 256, kBcWarps = kBcThreads / 32, kBcPer = 16, kBcTile = kBcThreads * kBcPer;
-constexpr int kBcCap = 1024;             // entries of a part that wait to be ranked
-constexpr int kBjThreads = 512, kBjWarps = kBjThreads / 32;
-
-// A logit and its token as one number: the larger logit is better, of equals the lower token.  0: none; NaN and -inf never enter.
-typedef unsigned long long Rank;
-constexpr uint32_t kNoKey = 0x007fffffu;              // float_to_key(-inf)
-__device__ __forceinline__ Rank rank_of(float x, int idx) { return (Rank)float_to_key(x + 0.f) << 32 | (uint32_t)~idx; }   // -0 is 0
-__device__ __forceinline__ uint32_t rank_key(Rank r) { return (uint32_t)(r >> 32); }
-__device__ __forceinline__ int rank_idx(Rank r) { return (int)~(uint32_t)r; }
+constexpr int kBcThreads = 256, kBcWarps = kBcThreads / 32, kBcPer = 16, kBcTile = kBcThreads * kBcPer, kBcBlocks = 4;
+constexpr int kBcChunk = 32 * kBcPer;    // logits of a warp's turn, consecutive ones
+constexpr int kBjThreads = 512, kBjWarps = kBjThreads / 32, kBjHold = 4;
+constexpr int kBjCap = 1024;             // entries that wait to be ranked
 
 // A row's part: the sum of e^x over its logits as sum * 2^n * e^base (NaN: a logit was NaN or +inf).
 struct BeamPart { double sum; int32_t n; float base; };
 
-// p += v.
 __device__ __forceinline__ double pow2(float e) { return e < -1000.f ? 0.0 : __longlong_as_double((long long)((int)e + 1023) << 52); }   // whole e <= 0
+__device__ __noinline__ double exp_of(double v) { return exp(v); }                     // hardly ever called
+// p += v.
 __device__ __forceinline__ void join_sums(BeamPart& p, const BeamPart& v) {
   if (v.sum == 0.0) return;
   if (p.sum == 0.0) { p = v; return; }
@@ -38,260 +34,117 @@ __device__ __forceinline__ void join_sums(BeamPart& p, const BeamPart& v) {
     return;
   }
   const double rp = (double)p.base + p.n * 0.6931471805599453, rv = (double)v.base + v.n * 0.6931471805599453;
-  if (rp >= rv) { p.sum += v.sum * exp(rv - rp); return; }
-  const double mine = p.sum * exp(rp - rv);
+  if (rp >= rv) { p.sum += v.sum * exp_of(rv - rp); return; }
+  const double mine = p.sum * exp_of(rp - rv);
   p = v;
   p.sum += mine;
 }
-
 __device__ __forceinline__ BeamPart other_part(const BeamPart& p, int o) {
   return {__shfl_xor_sync(0xffffffffu, p.sum, o), __shfl_xor_sync(0xffffffffu, p.n, o), __shfl_xor_sync(0xffffffffu, p.base, o)};
 }
 
-// The `want`-th best of a warp's lanes, each with one entry; 0 where there are fewer.
-__device__ __forceinline__ Rank warp_nth(Rank mine, int want) {
-  uint32_t key = 0u, low = 0u;
-  for (int i = 0; i < want; ++i) {
-    key = __reduce_max_sync(0xffffffffu, rank_key(mine));
-    if (key <= kNoKey) return 0ull;
-    low = __reduce_max_sync(0xffffffffu, rank_key(mine) == key ? (uint32_t)mine : 0u);
-    if (mine == ((Rank)key << 32 | low)) mine = 0ull;
-  }
-  return (Rank)key << 32 | low;
-}
-
-__device__ __forceinline__ float max_nan(float a, float b) {
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
   float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float ex2_part(float f) {      // |f| <= 1/2
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(f));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 
+// The logits of a warp's turn: lane by lane, so that a row may start anywhere and is summed in the same order wherever it does.
 template <typename T>
-__device__ __forceinline__ void load_tile(const T* x_row, int t, int v1, float (&x)[kBcPer]) {
-  if (t + kBcTile <= v1) {
+__device__ __forceinline__ void load_chunk(const T* x_row, int i0, int v1, float (&x)[kBcPer]) {
+  const int lane = threadIdx.x & 31;
+  if (i0 + kBcChunk <= v1) {
 #pragma unroll
-    for (int j = 0; j < kBcPer; ++j) x[j] = to_f(x_row[t + j * kBcThreads + (int)threadIdx.x]);
+    for (int j = 0; j < kBcPer; ++j) x[j] = to_f(x_row[i0 + j * 32 + lane]);
   } else {
 #pragma unroll
-    for (int j = 0; j < kBcPer; ++j) {
-      const int i = t + j * kBcThreads + (int)threadIdx.x;
-      x[j] = i < v1 ? to_f(x_row[i]) : -INFINITY;
-    }
+    for (int j = 0; j < kBcPer; ++j) x[j] = i0 + j * 32 + lane < v1 ? to_f(x_row[i0 + j * 32 + lane]) : -INFINITY;
   }
 }
 
-struct BeamScratch { Rank list[2][kBeamMaxK], fresh[kBcCap], post[kBcWarps]; int count; };
-
-// Entries 0 .. n-1 of s.fresh join the `have` of s.list[cur], which are in order: each one's place is the number of better ones.
-__device__ __forceinline__ void rank_entries(BeamScratch& s, int n, int k, int& have, int& cur) {
-  for (int i = threadIdx.x; i < have + n; i += kBcThreads) {
-    const Rank mine = i < have ? s.list[cur][i] : s.fresh[i - have];
-    int place = i < have ? i : 0;
-    if (i >= have) for (int o = 0; o < have; ++o) place += s.list[cur][o] > mine;
-#pragma unroll 4
-    for (int o = 0; o < n; ++o) place += s.fresh[o] > mine;
-    if (place < k) s.list[cur ^ 1][place] = mine;
-  }
-  cur ^= 1;
-  have = min(k, have + n);
-  __syncthreads();
-}
-
-// The k best of a part whatever its order, tile by tile, where too many entries passed the bound on the way (rows that rise towards their
-// end, masks that leave a warp without logits): 64 beams over 12,345 sorted logits take 1.7 times as long as unsorted ones.
+// One pass over the logits: every row's sum, and the largest logit of every 512.  The k best of a question lie in the k chunks with the
+// best largest logits (any other chunk has k logits above its own largest, or equal and at lower tokens), so nothing else is kept:
+// ranking on the way, by bounds from what the block had seen, took 45 us for 48 x 4 rows of 151,936 where this takes 22.  The loads of a warp's
+// next chunk are in flight while it works on one.
 template <typename T>
-__device__ __noinline__ int ordered_best(const T* x_row, int v0, int v1, int k, BeamScratch& s) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, want = (k + kBcWarps - 1) / kBcWarps;
-  int have = 0, cur = 0;
-  Rank kth = 0ull;                                          // what a newcomer has to beat
-  for (int t = v0; t < v1; t += kBcTile) {
-    float x[kBcPer];
-    load_tile(x_row, t, v1, x);
-    Rank best = 0ull;
-#pragma unroll
-    for (int j = 0; j < kBcPer; ++j) {
-      const Rank e = rank_of(x[j], t + j * kBcThreads + (int)threadIdx.x);
-      if (x[j] > -INFINITY && e > best) best = e;
-    }
-    const Rank post = warp_nth(best, want);
-    __syncthreads();
-    if (lane == 0) s.post[warp] = post;
-    if (threadIdx.x == 0) s.count = 0;
-    __syncthreads();
-    Rank bound = s.post[0];
-#pragma unroll
-    for (int w = 1; w < kBcWarps; ++w) bound = min(bound, s.post[w]);
-#pragma unroll
-    for (int j = 0; j < kBcPer; ++j) {
-      const Rank e = rank_of(x[j], t + j * kBcThreads + (int)threadIdx.x);
-      if (x[j] > -INFINITY && e > kth && e >= bound) {
-        const int at = atomicAdd(&s.count, 1);
-        if (at < kBcCap) s.fresh[at] = e;
-      }
-    }
-    __syncthreads();
-    int n = s.count;
-    if (n > kBcCap) {                                       // the bound says nothing: one at a time, each the best behind the one before
-      Rank last = ~0ull;
-      for (n = 0; n < k; ++n) {
-        best = 0ull;
-#pragma unroll
-        for (int j = 0; j < kBcPer; ++j) {
-          const Rank e = rank_of(x[j], t + j * kBcThreads + (int)threadIdx.x);
-          if (x[j] > -INFINITY && e > kth && e < last && e > best) best = e;
-        }
-        best = warp_nth(best, 1);
-        __syncthreads();
-        if (lane == 0) s.post[warp] = best;
-        __syncthreads();
-        last = s.post[0];
-#pragma unroll
-        for (int w = 1; w < kBcWarps; ++w) last = max(last, s.post[w]);
-        if (last == 0ull) break;
-        if (threadIdx.x == 0) s.fresh[n] = last;
-      }
-      __syncthreads();
-    }
-    rank_entries(s, n, k, have, cur);
-    if (have == k) kth = s.list[cur][k - 1];
-  }
-  if (cur) {
-    for (int i = threadIdx.x; i < have; i += kBcThreads) s.list[0][i] = s.list[1][i];
-    __syncthreads();
-  }
-  return have;
-}
-
-// One block per part of a row.  Its warps walk the part's tiles without waiting for one another: each keeps its lanes' best logits and
-// publishes the want-th of them, want = ceil(k / 8), so that the least of the eight is a bound that k logits reach; what reaches it is
-// set aside, some 2.5 k (1 + log tiles) entries, and ranked at the end.  The next tile's loads are in flight meanwhile.
-template <typename T>
-__global__ void __launch_bounds__(kBcThreads, 3)
-beam_rows_kernel(const T* __restrict__ logits, long long stride, const float* __restrict__ scores, int vocab, int splits, int tiles_per_split, int k,
-                 BeamPart* __restrict__ parts, Rank* __restrict__ best) {
-  __shared__ BeamScratch s;
-  __shared__ double s_sum[kBcWarps];
-  __shared__ int s_n[kBcWarps];
-  __shared__ float s_base[kBcWarps];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+__global__ void __launch_bounds__(kBcThreads, kBcBlocks)
+beam_rows_kernel(const T* __restrict__ logits, long long stride, const float* __restrict__ scores, int vocab, int chunks, int splits, int tiles_per_split,
+                 BeamPart* __restrict__ parts, float* __restrict__ largest) {
+  __shared__ BeamPart s_part[kBcWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long row = blockIdx.x / splits, part = blockIdx.x;
   const int v0 = (int)(blockIdx.x % splits) * tiles_per_split * kBcTile, v1 = (int)min((long long)vocab, (long long)v0 + (long long)tiles_per_split * kBcTile);
-  Rank* out = best + part * k;
-  if (!(fabsf(scores[row]) < INFINITY)) {                    // a beam without a score offers nothing
-    if (tid < k) out[tid] = 0ull;
-    if (tid == 0) parts[part] = {0.0, 0, 0.f};
-    return;
-  }
+  float* out = largest + row * chunks;
   const T* x_row = logits + row * stride;
-  const int want = (k + kBcWarps - 1) / kBcWarps;
-  float x[kBcPer];
-  load_tile(x_row, v0, v1, x);
-  if (tid == 0) s.count = 0;
-  float mine = -INFINITY;                                   // this lane's best, its token, and the warp's best
-  int mine_at = 0;
-  uint32_t top = 0u;
-  float base = 0.f, big_n = 0.f;                            // the warp's reference
+  const bool live = fabsf(scores[row]) < INFINITY;            // a beam without a score offers nothing
+  float top = -INFINITY, base = 0.f, big_n = 0.f, floor_x = 0.f;   // the warp's largest logit, its sum's reference, and what vanishes beside it
   double sum = 0.0;
   bool nan = false;
-  for (int t = v0; t < v1; t += kBcTile) {
-    float nx[kBcPer];
-    if (t + kBcTile < v1) load_tile(x_row, t + kBcTile, v1, nx);
-    float m = x[0], m2 = x[1];
+  auto step = [&](const float (&x)[kBcPer], int i0) {
+    float m = max3_nan(x[0], x[1], x[2]), m2 = max3_nan(x[3], x[4], x[5]);
 #pragma unroll
-    for (int j = 2; j < kBcPer; j += 2) { m = max_nan(m, x[j]); m2 = max_nan(m2, x[j + 1]); }
-    m = max_nan(m, m2);
-    if (m != m) {                                           // the maximum that passes over NaN
-      nan = true;
-      m = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < kBcPer; ++j) m = fmaxf(m, x[j]);
+    for (int j = 6; j + 4 <= kBcPer; j += 4) { m = max3_nan(m, x[j], x[j + 1]); m2 = max3_nan(m2, x[j + 2], x[j + 3]); }
+    m = max3_nan(m, m2, max3_nan(m2, x[kBcPer - 2], x[kBcPer - 1]));
+    if (m != m) { nan = true; m = -INFINITY; }                 // the row counts for nothing
+    m = key_to_float(__reduce_max_sync(0xffffffffu, float_to_key(m)));
+    if (lane == 0) out[i0 / kBcChunk] = m;
+    if (m > top) {
+      // The sum is kept relative to a power of two, which moves no bit of a term (and to e^base for logits beyond 1e6).
+      const float new_base = fabsf(m) < 1e6f ? 0.f : m, new_n = rintf((m - new_base) * 1.44269504f);
+      if (sum != 0.0) sum *= new_base == 0.f && base == 0.f ? pow2(big_n - new_n) : exp_of(((double)base - new_base) + ((double)big_n - new_n) * 0.6931471805599453);
+      top = m; base = new_base; big_n = new_n; floor_x = m - 80.f;
     }
-    if (__any_sync(0xffffffffu, m > mine)) {
-      if (m > mine) {
-        mine = m;
+    if (top == -INFINITY) return;
+    // e^x / 2^big_n: the exponent's whole part by integer arithmetic, the fraction (exact to 2^-25) by ex2; two at a time.
+    if (base == 0.f) {
+      const float magic = 12582912.f - big_n;
+      const unsigned long long log2e = f32x2(1.44269504f, 1.44269504f), rest = f32x2(1.92596299e-8f, 1.92596299e-8f), magic2 = f32x2(magic, magic),
+                               minus = f32x2(-1.f, -1.f);
+      unsigned long long a = 0ull, b = 0ull;
 #pragma unroll
-        for (int j = kBcPer - 1; j >= 0; --j) if (x[j] == m) mine_at = t + j * kBcThreads + tid;
+      for (int j = 0; j < kBcPer; j += 2) {
+        // e^-80 of the largest is nothing in the sum's 53 bits, and -inf may count as that
+        const unsigned long long y = f32x2(fmaxf(x[j], floor_x), fmaxf(x[j + 1], floor_x));
+        const unsigned long long r = fma_f32x2(y, log2e, magic2), n = fma_f32x2(r, minus, magic2);
+        float f0, f1, r0, r1;
+        f32x2_split(fma_f32x2(y, rest, fma_f32x2(y, log2e, n)), f0, f1);
+        f32x2_split(r, r0, r1);
+        const unsigned long long e = f32x2(__int_as_float(__float_as_int(ex2_approx(f0)) + (__float_as_int(r0) << 23)),
+                                           __int_as_float(__float_as_int(ex2_approx(f1)) + (__float_as_int(r1) << 23)));
+        if (j & 2) b = add_f32x2(b, e); else a = add_f32x2(a, e);
       }
-      const Rank post = warp_nth(mine > -INFINITY ? rank_of(mine, mine_at) : 0ull, want);
-      if (lane == 0) *(volatile Rank*)&s.post[warp] = post;
-      const uint32_t t_max = __reduce_max_sync(0xffffffffu, float_to_key(m));
-      if (t_max > top) {
-        // The sum is kept relative to a power of two, which moves no bit of a term (and to e^base for logits beyond 1e6).
-        const float mx = key_to_float(t_max), new_base = fabsf(mx) < 1e6f ? 0.f : mx, new_n = rintf((mx - new_base) * 1.44269504f);
-        if (sum != 0.0) sum *= new_base == 0.f && base == 0.f ? pow2(big_n - new_n) : exp(((double)base - new_base) + ((double)big_n - new_n) * 0.6931471805599453);
-        top = t_max; base = new_base; big_n = new_n;
-      }
-    } else if (t == v0 && lane == 0) {
-      s.post[warp] = 0ull;                                  // nothing but -inf
+      float s0, s1;
+      f32x2_split(add_f32x2(a, b), s0, s1);
+      sum += (double)(s0 + s1);
+    } else {                                                // big_n is 0
+      float a = 0.f;
+#pragma unroll
+      for (int j = 0; j < kBcPer; ++j) a += x[j] >= floor_x ? expf(x[j] - base) : 0.f;
+      sum += (double)a;
     }
-    if (t == v0) __syncthreads();                           // later a bound that is behind lets a few more pass
-    Rank bound = *(volatile Rank*)&s.post[0];
-#pragma unroll
-    for (int w = 1; w < kBcWarps; ++w) bound = min(bound, *(volatile Rank*)&s.post[w]);
-    const float least = rank_key(bound) > kNoKey ? key_to_float(rank_key(bound)) : -INFINITY;
-    if (m >= least) {
-#pragma unroll
-      for (int j = 0; j < kBcPer; ++j)
-        if (x[j] >= least) {
-          const Rank e = rank_of(x[j], t + j * kBcThreads + tid);
-          if (e >= bound && x[j] > -INFINITY) {
-            const int at = atomicAdd(&s.count, 1);
-            if (at < kBcCap) s.fresh[at] = e;
-          }
-        }
+  };
+  int i = v0 + warp * kBcChunk;
+  if (live && i < v1) {
+    float x[kBcPer], y[kBcPer];
+    load_chunk(x_row, i, v1, x);
+    for (;;) {
+      if (i + kBcTile < v1) load_chunk(x_row, i + kBcTile, v1, y);
+      step(x, i);
+      i += kBcTile;
+      if (i >= v1) break;
+      if (i + kBcTile < v1) load_chunk(x_row, i + kBcTile, v1, x);
+      step(y, i);
+      i += kBcTile;
+      if (i >= v1) break;
     }
-    if (top > kNoKey) {
-      // e^x / 2^big_n: the exponent's whole part by integer arithmetic, the fraction (exact to 2^-25) by ex2.
-      const float floor_x = key_to_float(top) - 80.f, magic = 12582912.f - big_n;
-      float a = 0.f, b = 0.f;
-      if (base == 0.f) {
-#pragma unroll
-        for (int j = 0; j < kBcPer; ++j) {
-          const float y = fmaxf(x[j], floor_x);             // e^-80 of the largest is nothing in the sum's 53 bits, and -inf may count as that
-          const float r = fmaf(y, 1.44269504f, magic), f = fmaf(y, 1.92596299e-8f, fmaf(y, 1.44269502f, magic - r));
-          const float e = __int_as_float(__float_as_int(ex2_part(f)) + (__float_as_int(r) << 23));
-          if (j & 1) b += e; else a += e;
-        }
-      } else {                                              // big_n is 0
-#pragma unroll
-        for (int j = 0; j < kBcPer; ++j) a += x[j] >= floor_x ? expf(x[j] - base) : 0.f;
-      }
-      sum += (double)(a + b);
-    }
-#pragma unroll
-    for (int j = 0; j < kBcPer; ++j) x[j] = nx[j];
   }
-  if (nan || top >= float_to_key(INFINITY)) sum = __longlong_as_double(0x7ff8000000000000ll);
+  if (__any_sync(0xffffffffu, nan) || top == INFINITY) sum = __longlong_as_double(0x7ff8000000000000ll);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (lane == 0) { s_sum[warp] = sum; s_n[warp] = (int)big_n; s_base[warp] = base; }
+  if (lane == 0) s_part[warp] = {sum, (int)big_n, base};
   __syncthreads();
-  int n = s.count, have = 0, cur = 0;
-  if (n > kBcCap) {
-    have = ordered_best(x_row, v0, v1, k, s);
-  } else {
-    // What reaches the bound of all tiles is what remains: every thread holds up to four of the entries meanwhile.
-    Rank bound = s.post[0], keep[kBcCap / kBcThreads];
-#pragma unroll
-    for (int w = 1; w < kBcWarps; ++w) bound = min(bound, s.post[w]);
-#pragma unroll
-    for (int i = 0; i < kBcCap / kBcThreads; ++i) keep[i] = i * kBcThreads + tid < n ? s.fresh[i * kBcThreads + tid] : 0ull;
-    __syncthreads();
-    if (tid == 0) s.count = 0;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kBcCap / kBcThreads; ++i) if (keep[i] != 0ull && keep[i] >= bound) s.fresh[atomicAdd(&s.count, 1)] = keep[i];
-    __syncthreads();
-    rank_entries(s, s.count, k, have, cur);
-  }
-  if (tid < k) out[tid] = tid < have ? s.list[cur][tid] : 0ull;
-  if (warp == kBcWarps - 1) {
-    BeamPart p = {s_sum[lane % kBcWarps], s_n[lane % kBcWarps], s_base[lane % kBcWarps]};
+  if (warp == 0) {
+    BeamPart p = s_part[lane % kBcWarps];
 #pragma unroll
     for (int o = 1; o < kBcWarps; o <<= 1) join_sums(p, other_part(p, o));
     if (lane == 0) parts[part] = p;
@@ -306,123 +159,186 @@ __device__ __forceinline__ unsigned long long score_key(double v) {
 __device__ __forceinline__ double key_score(unsigned long long k) {
   return __longlong_as_double((long long)(k >> 63 ? k & 0x7fffffffffffffffull : ~k));
 }
-// at: beam * vocab + token; key 0: none.  Equals go to the lower beam; within a beam, whose scores may be equal although its logits are
-// not, to the larger logit, as in the choice of the row's best, and then to the lower token.
+// at: beam * vocab + token (or a chunk's first token); key 0: none.  Equals go to the lower beam; within a beam, whose scores may be equal
+// although its logits are not, to the larger logit, and then to the lower token.
 struct BeamScore { unsigned long long key; int32_t at; uint32_t logit; };
 constexpr BeamScore kNoScore = {0ull, 0x7fffffff, 0u};
+__device__ __noinline__ bool equal_before(int a_at, uint32_t a_logit, int b_at, uint32_t b_logit, int vocab) {
+  return a_logit != b_logit && a_at / vocab == b_at / vocab ? a_logit > b_logit : a_at < b_at;
+}
 struct BeamOrder {
   int vocab;
   __device__ __forceinline__ bool operator()(const BeamScore& a, const BeamScore& b) const {
-    if (a.key != b.key) return a.key > b.key;
-    return a.logit != b.logit && a.at / vocab == b.at / vocab ? a.logit > b.logit : a.at < b.at;
+    return a.key > b.key || (a.key == b.key && a.at != b.at && equal_before(a.at, a.logit, b.at, b.logit, vocab));
   }
 };
-__device__ __forceinline__ BeamScore warp_best(BeamScore v, const BeamOrder& better) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    BeamScore w;
-    w.key = __shfl_xor_sync(0xffffffffu, v.key, o);
-    w.at = __shfl_xor_sync(0xffffffffu, v.at, o);
-    w.logit = __shfl_xor_sync(0xffffffffu, v.logit, o);
-    if (better(w, v)) v = w;
+struct BeamQuestion {
+  double lse[kBeamMax], score[kBeamMax];
+  float least[kBeamMax];                                       // logits below it do not reach the bound
+  BeamScore fresh[kBjCap], best[kBeamMaxK], one[kBjWarps];
+  uint32_t post[kBjWarps];
+  int count;
+  __device__ __forceinline__ BeamScore of(float x, int b, int at) const {
+    if (!(x > -INFINITY)) return kNoScore;
+    x += 0.f;                                                  // -0 is 0
+    const double v = score[b] + ((double)x - lse[b]);
+    return v > -INFINITY && v < INFINITY ? BeamScore{score_key(v), at, float_to_key(x)} : kNoScore;
   }
-  return v;
+  // 64-bit scores are for the few logits that may count: the others stay below a logit that gives less than `v`.  1e-12 of the
+  // numbers involved is far more than those scores' own rounding.
+  __device__ __forceinline__ void reach(double v, int b) {
+    const double x = v - score[b] + lse[b];
+    least[b] = __double2float_rd(x - 1e-12 * (fabs(v) + fabs(score[b]) + fabs(lse[b])));
+  }
+};
+
+// The k best of what `each` hands to its argument, in order, into s.best; their number.
+template <typename Each>
+__device__ __forceinline__ int k_best(BeamQuestion& s, const BeamOrder& better, int k, const Each& each) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) s.count = 0;
+  __syncthreads();
+  each([&](const BeamScore& v) {
+    const int at = atomicAdd(&s.count, 1);
+    if (at < kBjCap) s.fresh[at] = v;
+  });
+  __syncthreads();
+  int have = s.count;
+  if (have > kBjCap) {                                        // equal scores, or chunks in order, by the hundred: one at a time
+    BeamScore last{~0ull, -1, ~0u};
+    for (have = 0; have < k; ++have) {
+      BeamScore mine = kNoScore;
+      each([&](const BeamScore& v) { if (better(last, v) && better(v, mine)) mine = v; });
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        const BeamScore w = {__shfl_xor_sync(0xffffffffu, mine.key, o), __shfl_xor_sync(0xffffffffu, mine.at, o), __shfl_xor_sync(0xffffffffu, mine.logit, o)};
+        if (better(w, mine)) mine = w;
+      }
+      if (lane == 0) s.one[warp] = mine;
+      __syncthreads();
+      mine = s.one[0];
+      for (int w = 1; w < kBjWarps; ++w) if (better(s.one[w], mine)) mine = s.one[w];
+      __syncthreads();
+      if (!mine.key) break;
+      if (tid == 0) s.best[have] = mine;
+      last = mine;
+    }
+  } else {
+    for (int i = tid / 4; i < (have + 7) / 8 * 8; i += kBjThreads / 4) {      // four lanes count an entry's betters
+      const BeamScore v = i < have ? s.fresh[i] : kNoScore;
+      int place = 0;
+      if (i < have)
+        for (int o = tid % 4; o < have; o += 4) place += better(s.fresh[o], v);
+      place += __shfl_xor_sync(0xffffffffu, place, 1);
+      place += __shfl_xor_sync(0xffffffffu, place, 2);
+      if (i < have && tid % 4 == 0 && place < k) s.best[place] = v;
+    }
+    have = min(have, k);
+  }
+  __syncthreads();
+  return have;
 }
 
 struct BeamChoiceOut { float* score; int32_t *beam, *token; float* live_score; int32_t *live_beam, *live_token; };
 
-// One block per question.  Scores are 64-bit; a bound from below, in 32 bits rounded down, leaves a few times k candidates to rank.
+// One block per question: the rows' sums, the k best chunks by their largest logits, and the k best of what lies in those.
+template <typename T>
 __global__ void __launch_bounds__(kBjThreads)
-beam_join_kernel(const BeamPart* parts, const Rank* best, const float* scores, int beams, int vocab, int splits, int k, const int32_t* stop, int n_stop,
-                 const BeamChoiceOut out) {
+beam_join_kernel(const BeamPart* parts, const float* largest, const T* logits, long long stride, const float* scores, int beams, int vocab, int chunks,
+                 int splits, int k, const int32_t* stop, int n_stop, const BeamChoiceOut out) {
   grid_dependency_wait();
+  __shared__ BeamQuestion s;
   __shared__ BeamPart s_part[kBeamMax];
-  __shared__ double s_lse[kBeamMax], s_score[kBeamMax];
-  __shared__ BeamScore s_new[kBcCap], s_one[kBjWarps], s_done[kBeamMaxK];
-  __shared__ uint32_t s_post[kBjWarps];
-  __shared__ int s_count;
+  __shared__ BeamScore s_chunk[kBeamMaxK];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const long long q = blockIdx.x;
   const BeamOrder better{vocab};
-  if (tid == 0) s_count = 0;
+  // The chunks are dealt to the warps one by one, so that every warp sees some of every beam; a thread's first few are fetched here.
+  const int n = beams * chunks, c0 = lane * kBjWarps + warp;
+  float hold[kBjHold];
+#pragma unroll
+  for (int i = 0; i < kBjHold; ++i) hold[i] = i * kBjThreads + c0 < n ? largest[q * n + i * kBjThreads + c0] : -INFINITY;
   for (int b = warp; b < beams; b += kBjWarps) {
     BeamPart p = {0.0, 0, 0.f};
     for (int i = lane; i < splits; i += 32) join_sums(p, parts[(q * beams + b) * splits + i]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) join_sums(p, other_part(p, o));
+    for (int o = 1; o < 32 && o < splits; o <<= 1) join_sums(p, other_part(p, o));
     if (lane == 0) s_part[b] = p;
   }
   __syncthreads();
   if (tid < beams) {                                          // nothing summed, or NaN: no candidates below
     const BeamPart p = s_part[tid];
-    s_lse[tid] = ((double)p.base + (double)p.n * 0.6931471805599453) + log(p.sum);
-    s_score[tid] = (double)scores[q * beams + tid];
+    s.lse[tid] = ((double)p.base + (double)p.n * 0.6931471805599453) + log(p.sum);
+    s.score[tid] = p.sum > 0.0 ? (double)scores[q * beams + tid] : -INFINITY;
+    s.least[tid] = p.sum > 0.0 ? (float)(s.score[tid] - s.lse[tid]) : -INFINITY;        // what turns logits into scores, for now
   }
   __syncthreads();
-  // Candidates are taken the parts' best ones first, so that every warp sees some of those.
-  const int lists = beams * splits, n = lists * k;
-  const Rank* ranks = best + q * n;
-  auto candidate = [&](int c) -> BeamScore {
-    const int place = c / lists, list = c - place * lists, b = list / splits;
-    const Rank r = ranks[list * k + place];
-    if (r == 0ull) return kNoScore;
-    const double v = s_score[b] + ((double)key_to_float(rank_key(r)) - s_lse[b]);
-    return v > -INFINITY && v < INFINITY ? BeamScore{score_key(v), b * vocab + rank_idx(r), rank_key(r)} : kNoScore;
+  const float per_chunk = 1.f / (float)chunks;
+  auto beam_of = [&](int c) {
+    const int b = (int)(((float)c + 0.5f) * per_chunk);
+    return c < b * chunks ? b - 1 : c >= (b + 1) * chunks ? b + 1 : b;
   };
-  unsigned long long top = 0ull;
-  for (int c = tid; c < n; c += kBjThreads) top = max(top, candidate(c).key);
-  uint32_t key = top ? float_to_key(__double2float_rd(key_score(top))) : 0u, post = 0u;
-  const int warps = min(kBjWarps, (n + 31) / 32);               // those with candidates: each has `want` that reach the bound
+  // A bound from below: every warp's `want`-th best thread by the best of its chunks, and the least of those; in 32 bits, less more
+  // than their rounding (two roundings of numbers no larger than these, 2^-24 each).
+  float top = -INFINITY, size = 0.f;
+  auto see = [&](float x, int c) {
+    const float off = s.least[beam_of(c)], v = x + off;
+    if (v > top) { top = v; size = fabsf(off) + fabsf(v); }
+  };
+#pragma unroll
+  for (int i = 0; i < kBjHold; ++i) if (i * kBjThreads + c0 < n) see(hold[i], i * kBjThreads + c0);
+  for (int c = kBjHold * kBjThreads + c0; c < n; c += kBjThreads) see(largest[q * n + c], c);
+  top -= size * 2.4e-7f;
+  uint32_t key = top > -INFINITY && top < INFINITY ? float_to_key(top) : 0u, post = 0u;
+  const int warps = min(kBjWarps, n);                          // those with chunks: each has `want` threads that reach the bound
   for (int i = 0, want = (k + warps - 1) / warps; i < want; ++i) {
     post = __reduce_max_sync(0xffffffffu, key);
     const unsigned who = __ballot_sync(0xffffffffu, key == post);
     if (lane == __ffs(who) - 1) key = 0u;
   }
-  if (lane == 0) s_post[warp] = post;
+  if (lane == 0) s.post[warp] = post;
   __syncthreads();
-  uint32_t bound = s_post[0];
-  for (int w = 1; w < warps; ++w) bound = min(bound, s_post[w]);
-  const unsigned long long least = bound ? score_key((double)key_to_float(bound)) : 1ull;
-  for (int c = tid; c < n; c += kBjThreads) {
-    const BeamScore v = candidate(c);
-    if (v.key >= least) {
-      const int at = atomicAdd(&s_count, 1);
-      if (at < kBcCap) s_new[at] = v;
-    }
+  if (tid < beams) {
+    uint32_t bound = s.post[0];
+    for (int w = 1; w < warps; ++w) bound = min(bound, s.post[w]);
+    if (bound) s.reach((double)key_to_float(bound), tid); else s.least[tid] = -INFINITY;
+    if (!(s.score[tid] > -INFINITY)) s.least[tid] = INFINITY;
   }
   __syncthreads();
-  int have = s_count;
-  if (have > kBcCap) {                                        // equal scores by the hundred: one at a time
-    BeamScore last{~0ull, -1, ~0u};
-    for (have = 0; have < k; ++have) {
-      BeamScore mine = kNoScore;
-      for (int c = tid; c < n; c += kBjThreads) {
-        const BeamScore v = candidate(c);
-        if (v.key && better(last, v) && better(v, mine)) mine = v;
+  auto take = [&](float x, int c, auto&& use) {
+    const int b = beam_of(c);
+    if (x >= s.least[b] && x < INFINITY) {
+      const BeamScore v = s.of(x, b, b * vocab + (c - b * chunks) * kBcChunk);
+      if (v.key) use(v);
+    }
+  };
+  const int picked = k_best(s, better, k, [&](auto&& use) {
+#pragma unroll
+    for (int i = 0; i < kBjHold; ++i) if (i * kBjThreads + c0 < n) take(hold[i], i * kBjThreads + c0, use);
+    for (int c = kBjHold * kBjThreads + c0; c < n; c += kBjThreads) take(largest[q * n + c], c, use);
+  });
+  // The k-th chunk's largest is one of k logits that reach it.
+  if (tid < picked) s_chunk[tid] = s.best[tid];
+  if (tid < beams && picked == k) s.reach(key_score(s.best[k - 1].key), tid);
+  __syncthreads();
+  const int have = k_best(s, better, k, [&](auto&& use) {
+    for (int c = warp; c < picked; c += kBjWarps) {
+      const int b = s_chunk[c].at / vocab, i0 = s_chunk[c].at - b * vocab;
+      const float least = s.least[b];
+      const T* x_row = logits + (q * beams + b) * stride;
+      float x[kBcPer];
+      load_chunk(x_row, i0, vocab, x);
+      uint32_t hits = 0u;
+#pragma unroll
+      for (int j = 0; j < kBcPer; ++j) hits |= x[j] >= least ? 1u << j : 0u;
+      for (; hits; hits &= hits - 1u) {                        // few: read again rather than held in a register each
+        const int i = i0 + (__ffs(hits) - 1) * 32 + lane;
+        const BeamScore v = s.of(i < vocab ? to_f(x_row[i]) : -INFINITY, b, b * vocab + i);
+        if (v.key) use(v);
       }
-      mine = warp_best(mine, better);
-      if (lane == 0) s_one[warp] = mine;
-      __syncthreads();
-      mine = s_one[0];
-      for (int w = 1; w < kBjWarps; ++w) if (better(s_one[w], mine)) mine = s_one[w];
-      __syncthreads();
-      if (!mine.key) break;
-      if (tid == 0) s_done[have] = mine;
-      last = mine;
     }
-  } else {
-    for (int i = tid; i < have; i += kBjThreads) {
-      const BeamScore v = s_new[i];
-      int place = 0;
-#pragma unroll 4
-      for (int o = 0; o < have; ++o) place += better(s_new[o], v);
-      if (place < k) s_done[place] = v;
-    }
-    have = min(have, k);
-  }
-  __syncthreads();
+  });
   if (tid < k) {
-    const BeamScore v = s_done[tid];
+    const BeamScore v = s.best[tid];
     const bool on = tid < have;
     out.score[q * k + tid] = on ? (float)key_score(v.key) : -INFINITY;
     out.beam[q * k + tid] = on ? v.at / vocab : -1;
@@ -433,7 +349,7 @@ beam_join_kernel(const BeamPart* parts, const Rank* best, const float* scores, i
     for (int c0 = 0; c0 < have; c0 += 32) {
       const int c = c0 + lane;
       bool on = c < have;
-      const BeamScore v = on ? s_done[c] : BeamScore{0ull, 0, 0u};
+      const BeamScore v = on ? s.best[c] : BeamScore{0ull, 0, 0u};
       const int token = v.at % vocab;
       for (int i = 0; i < n_stop; ++i) on = on && stop[i] != token;
       const unsigned mask = __ballot_sync(0xffffffffu, on);
@@ -601,29 +517,40 @@ reorder_copy_kernel(const msa_lm_state_part* part, int n_part, const ReorderCopy
 }
 
 template <typename T>
-void launch_beam_rows(const void* logits, int64_t stride, const float* scores, int64_t rows, int vocab, int splits, int tiles_per_split, int k,
-                      BeamPart* parts, Rank* best, cudaStream_t st) {
-  beam_rows_kernel<T><<<(unsigned)(rows * splits), kBcThreads, 0, st>>>((const T*)logits, stride, scores, vocab, splits, tiles_per_split, k, parts, best);
+int launch_beam_topk(const void* logits, int64_t stride, const float* scores, int batch, int beams, int vocab, int chunks, int splits, int tiles_per_split, int k,
+                     const int32_t* stop, int n_stop, BeamPart* parts, float* largest, const BeamChoiceOut& out, cudaStream_t st) {
+  beam_rows_kernel<T><<<(unsigned)((int64_t)batch * beams * splits), kBcThreads, 0, st>>>((const T*)logits, stride, scores, vocab, chunks, splits,
+                                                                                         tiles_per_split, parts, largest);
+  MSA_LAUNCH_OK("beam_rows_kernel");
+  MSA_CUDA_OK(launch_kernel_pdl(beam_join_kernel<T>, dim3((unsigned)batch), dim3(kBjThreads), 0, st, true, parts, largest, (const T*)logits, stride, scores, beams,
+                                vocab, chunks, splits, k, stop, n_stop, out));
+  MSA_LAUNCH_OK("beam_join_kernel");
+  return MSA_OK;
 }
 
 }  // namespace msa
 
 using namespace msa;
 
-// Parts of a row: four blocks an SM, each of whole tiles.
+// Parts of a row, each of whole tiles: as many as let the blocks (kBcBlocks an SM at once) walk the fewest tiles one after the other, with one
+// more tile's time for a block's start and end.
 static int beam_splits(int64_t rows, int32_t vocab, int* tiles_per_split) {
   const int tiles = (vocab + kBcTile - 1) / kBcTile;
-  const int64_t want = (148 * 4 + rows - 1) / rows;
-  const int splits = (int)(want < tiles ? want : tiles);
-  *tiles_per_split = (tiles + splits - 1) / splits;
-  return (tiles + *tiles_per_split - 1) / *tiles_per_split;
+  int64_t best = 0;
+  int per = tiles;
+  for (int p = tiles; p >= 1; --p) {
+    const int64_t blocks = rows * ((tiles + p - 1) / p), cost = (blocks + kBcBlocks * 148 - 1) / (kBcBlocks * 148) * (p + 1);
+    if (best == 0 || cost < best) { best = cost; per = p; }
+  }
+  *tiles_per_split = per;
+  return (tiles + per - 1) / per;
 }
 
 extern "C" int64_t msa_lm_beam_topk_workspace(int32_t batch, int32_t beams, int32_t vocab, int32_t k) {
   if (batch <= 0 || beams <= 0 || vocab <= 0 || k <= 0) return 0;
   int per = 0;
   const int64_t parts = (int64_t)batch * beams * beam_splits((int64_t)batch * beams, vocab, &per);
-  return parts * ((int64_t)sizeof(BeamPart) + (int64_t)k * (int64_t)sizeof(Rank));
+  return parts * (int64_t)sizeof(BeamPart) + (int64_t)batch * beams * ((vocab + kBcChunk - 1) / kBcChunk) * 4;
 }
 
 extern "C" int msa_lm_beam_topk(const void* logits, int64_t stride, int32_t dtype, const float* scores, int32_t batch, int32_t beams, int32_t vocab,
@@ -642,15 +569,12 @@ extern "C" int msa_lm_beam_topk(const void* logits, int64_t stride, int32_t dtyp
   const int splits = beam_splits(rows, vocab, &per);
   MSA_REQUIRE(rows * splits < (1ll << 31), "beam_topk: too many rows");
   BeamPart* parts = (BeamPart*)workspace;
-  Rank* best = (Rank*)(parts + rows * splits);
-  cudaStream_t st = (cudaStream_t)stream;
-  MSA_LM_DISPATCH(dtype, { launch_beam_rows<T>(logits, stride, scores, rows, vocab, splits, per, k, parts, best, st); });
-  MSA_LAUNCH_OK("beam_rows_kernel");
+  float* largest = (float*)(parts + rows * splits);
   const BeamChoiceOut out{score, beam, token, live_score, live_beam, live_token};
-  MSA_CUDA_OK(launch_kernel_pdl(beam_join_kernel, dim3((unsigned)batch), dim3(kBjThreads), 0, st, true, parts, best, scores, beams, vocab, splits, k, stop,
-                                n_stop, out));
-  MSA_LAUNCH_OK("beam_join_kernel");
-  return MSA_OK;
+  MSA_LM_DISPATCH(dtype, {
+    return launch_beam_topk<T>(logits, stride, scores, batch, beams, vocab, (vocab + kBcChunk - 1) / kBcChunk, splits, per, k, stop, n_stop, parts, largest, out,
+                               (cudaStream_t)stream);
+  });
 }
 
 extern "C" int64_t msa_lm_reorder_workspace(int32_t batch, int32_t beams, int32_t n_part) {
