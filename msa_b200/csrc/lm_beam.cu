@@ -164,18 +164,22 @@ __device__ __forceinline__ double key_score(unsigned long long k) {
 struct BeamScore { unsigned long long key; int32_t at; uint32_t logit; };
 constexpr BeamScore kNoScore = {0ull, 0x7fffffff, 0u};
 __device__ __noinline__ bool equal_before(int a_at, uint32_t a_logit, int b_at, uint32_t b_logit, int vocab) {
-  return a_logit != b_logit && a_at / vocab == b_at / vocab ? a_logit > b_logit : a_at < b_at;
+  return a_at / vocab == b_at / vocab ? a_logit > b_logit : a_at < b_at;
 }
 struct BeamOrder {
   int vocab;
   __device__ __forceinline__ bool operator()(const BeamScore& a, const BeamScore& b) const {
-    return a.key > b.key || (a.key == b.key && a.at != b.at && equal_before(a.at, a.logit, b.at, b.logit, vocab));
+    if (a.key != b.key) return a.key > b.key;
+    return a.logit == b.logit ? a.at < b.at : equal_before(a.at, a.logit, b.at, b.logit, vocab);
   }
 };
 struct BeamQuestion {
   double lse[kBeamMax], score[kBeamMax];
   float least[kBeamMax];                                       // logits below it do not reach the bound
-  BeamScore fresh[kBjCap], best[kBeamMaxK], one[kBjWarps];
+  unsigned long long key[kBjCap];                              // entries that wait to be ranked: BeamScore, its parts side by side
+  int32_t at[kBjCap];
+  uint32_t logit[kBjCap];
+  BeamScore best[kBeamMaxK], one[kBjWarps];
   uint32_t post[kBjWarps];
   int count;
   __device__ __forceinline__ BeamScore of(float x, int b, int at) const {
@@ -199,8 +203,8 @@ __device__ __forceinline__ int k_best(BeamQuestion& s, const BeamOrder& better, 
   if (tid == 0) s.count = 0;
   __syncthreads();
   each([&](const BeamScore& v) {
-    const int at = atomicAdd(&s.count, 1);
-    if (at < kBjCap) s.fresh[at] = v;
+    const int i = atomicAdd(&s.count, 1);
+    if (i < kBjCap) { s.key[i] = v.key; s.at[i] = v.at; s.logit[i] = v.logit; }
   });
   __syncthreads();
   int have = s.count;
@@ -224,14 +228,23 @@ __device__ __forceinline__ int k_best(BeamQuestion& s, const BeamOrder& better, 
       last = mine;
     }
   } else {
-    for (int i = tid / 4; i < (have + 7) / 8 * 8; i += kBjThreads / 4) {      // four lanes count an entry's betters
-      const BeamScore v = i < have ? s.fresh[i] : kNoScore;
-      int place = 0;
-      if (i < have)
-        for (int o = tid % 4; o < have; o += 4) place += better(s.fresh[o], v);
+    // Each entry's place is the number of better ones; four lanes count for an entry.
+    for (int i = tid / 4; i < (have + 7) / 8 * 8; i += kBjThreads / 4) {
+      const unsigned long long mine = i < have ? s.key[i] : 0ull;
+      int place = 0, equal = 0;
+#pragma unroll 4
+      for (int o = tid % 4; o < have; o += 4) {
+        const unsigned long long other = s.key[o];
+        place += other > mine;
+        equal += other == mine;
+      }
+      if (equal > (i % 4 == tid % 4)) {                        // besides itself
+        const BeamScore v = {mine, s.at[i], s.logit[i]};
+        for (int o = tid % 4; o < have; o += 4) if (s.key[o] == mine) place += better(BeamScore{mine, s.at[o], s.logit[o]}, v);
+      }
       place += __shfl_xor_sync(0xffffffffu, place, 1);
       place += __shfl_xor_sync(0xffffffffu, place, 2);
-      if (i < have && tid % 4 == 0 && place < k) s.best[place] = v;
+      if (i < have && tid % 4 == 0 && place < k) s.best[place] = {mine, s.at[i], s.logit[i]};
     }
     have = min(have, k);
   }
@@ -277,8 +290,8 @@ beam_join_kernel(const BeamPart* parts, const float* largest, const T* logits, l
     const int b = (int)(((float)c + 0.5f) * per_chunk);
     return c < b * chunks ? b - 1 : c >= (b + 1) * chunks ? b + 1 : b;
   };
-  // A bound from below: every warp's `want`-th best thread by the best of its chunks, and the least of those; in 32 bits, less more
-  // than their rounding (two roundings of numbers no larger than these, 2^-24 each).
+  // A bound from below: every warp's `deep`-th best thread by the best of its chunks, and the `wide`-th best of the warps; in 32 bits, less
+  // more than their rounding (two roundings of numbers no larger than these, 2^-24 each).  It lets some 1.5 k chunks pass.
   float top = -INFINITY, size = 0.f;
   auto see = [&](float x, int c) {
     const float off = s.least[beam_of(c)], v = x + off;
@@ -289,19 +302,23 @@ beam_join_kernel(const BeamPart* parts, const float* largest, const T* logits, l
   for (int c = kBjHold * kBjThreads + c0; c < n; c += kBjThreads) see(largest[q * n + c], c);
   top -= size * 2.4e-7f;
   uint32_t key = top > -INFINITY && top < INFINITY ? float_to_key(top) : 0u, post = 0u;
-  const int warps = min(kBjWarps, n);                          // those with chunks: each has `want` threads that reach the bound
-  for (int i = 0, want = (k + warps - 1) / warps; i < want; ++i) {
+  const int warps = min(kBjWarps, n), most = max(1, warps * 13 / 16), deep = (k + most - 1) / most, wide = (k + deep - 1) / deep;
+  for (int i = 0; i < deep; ++i) {
     post = __reduce_max_sync(0xffffffffu, key);
     const unsigned who = __ballot_sync(0xffffffffu, key == post);
     if (lane == __ffs(who) - 1) key = 0u;
   }
   if (lane == 0) s.post[warp] = post;
   __syncthreads();
-  if (tid < beams) {
-    uint32_t bound = s.post[0];
-    for (int w = 1; w < warps; ++w) bound = min(bound, s.post[w]);
-    if (bound) s.reach((double)key_to_float(bound), tid); else s.least[tid] = -INFINITY;
-    if (!(s.score[tid] > -INFINITY)) s.least[tid] = INFINITY;
+  if (warp == 0) {
+    const uint32_t my_post = s.post[lane % kBjWarps];
+    int place = 0;
+    for (int w = 0; w < kBjWarps; ++w) place += s.post[w] > my_post || (s.post[w] == my_post && w < lane);
+    const uint32_t bound = __shfl_sync(0xffffffffu, my_post, __ffs(__ballot_sync(0xffffffffu, lane < kBjWarps && place == wide - 1)) - 1);
+    if (tid < beams) {
+      if (bound) s.reach((double)key_to_float(bound), tid); else s.least[tid] = -INFINITY;
+      if (!(s.score[tid] > -INFINITY)) s.least[tid] = INFINITY;
+    }
   }
   __syncthreads();
   auto take = [&](float x, int c, auto&& use) {
