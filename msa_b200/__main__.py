@@ -1,7 +1,8 @@
 """Command line.
 
     python -m msa_b200 generate --model DIR --prompt TEXT [--prompt TEXT ...] [--tokens 5,17,3 ...]
-                                [--max-new-tokens N] [--temperature T --top-p P --seed S] [--dtype float32] [--memory FILE] [--gpus N]
+                                [--max-new-tokens N] [--temperature T --top-p P --seed S] [--beams B --length-penalty L]
+                                [--dtype float32] [--memory FILE] [--gpus N]
     python -m msa_b200 designs            # the model designs the package serves
     python -m msa_b200 trace ...          # bin/trace_run
 """
@@ -23,7 +24,10 @@ def _generate(args) -> int:
     if design_of(args.model).serves == "memory" and (not args.memory or args.tokens):
         print("this model answers text prompts over a document memory: give --memory FILE and --prompt", file=sys.stderr)
         return 2
-    cfg = GenerateConfig(devices=list(range(args.gpus)), max_generate_tokens=args.max_new_tokens, temperature=args.temperature,
+    if design_of(args.model).serves == "memory" and args.beams != 1:
+        print("beam search is for models on state slots", file=sys.stderr)
+        return 2
+    cfg = GenerateConfig(num_beams=args.beams, length_penalty=args.length_penalty, devices=list(range(args.gpus)), max_generate_tokens=args.max_new_tokens, temperature=args.temperature,
                          top_p=args.top_p, seed=args.seed, max_context=args.max_context)
     with MSAEngine(cfg, ModelConfig(model_path=args.model, dtype=args.dtype), MemoryConfig(memory_file_path=args.memory or "")) as engine:
         texts, _, _ = engine.generate(prompts)
@@ -48,6 +52,8 @@ def main(argv=None) -> int:
     g.add_argument("--temperature", type=float, default=0.0)
     g.add_argument("--top-p", type=float, default=0.9)
     g.add_argument("--seed", type=int, default=None)
+    g.add_argument("--beams", type=int, default=1, help="beam search with that many beams (models on state slots)")
+    g.add_argument("--length-penalty", type=float, default=1.0)
     g.add_argument("--memory", default="", help="document file (memory models)")
     g.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"], help="models on state slots")
     g.add_argument("--gpus", type=int, default=1)

@@ -1,0 +1,81 @@
+"""Beam search over models on state slots: what a search remembers on the host.  The choice itself (``lm_ops.beam_topk``) and the moving
+of states (``SequenceStateCache.reorder_beams``) are kernels; ``scheduler.Scheduler`` drives them beside its other requests."""
+from __future__ import annotations
+
+import math
+from typing import Dict, List, Optional, Sequence, Tuple
+
+import torch
+
+from . import lm_ops as K
+
+
+class BeamSearch:
+    """One prompt's beams: their tokens and scores (sums of log probabilities), and the continuations that ended.
+
+    A continuation that ends counts while it is among the best ``beams``; an ended one is rated by its score divided by
+    ``tokens ** length_penalty``.  The search is over when the ``beams`` best that ended are rated no lower than the best live beam
+    would be by now, when no beam is left, or at ``max_new_tokens``, where live beams count as ended."""
+
+    def __init__(self, beams: int, max_new_tokens: int, stop: Sequence[int] = (), length_penalty: float = 1.0):
+        self.beams, self.max_new_tokens, self.length_penalty = beams, max_new_tokens, length_penalty
+        self.stop: Tuple[int, ...] = tuple(sorted(set(stop)))
+        self.tokens: List[List[int]] = [[] for _ in range(beams)]
+        self.scores: List[float] = [0.0] + [-math.inf] * (beams - 1)      # one prompt: one beam to begin with
+        self.ended: List[Tuple[float, List[int]]] = []                    # best first
+
+    def _rate(self, score: float, n: int) -> float:
+        return score / n ** self.length_penalty
+
+    def _end(self, score: float, tokens: List[int]) -> None:
+        self.ended.append((self._rate(score, len(tokens)), tokens))
+        self.ended.sort(key=lambda e: -e[0])                               # stable: equals stay in the order they came
+        del self.ended[self.beams:]
+
+    def update(self, candidates, live) -> bool:
+        """``candidates`` and ``live``: (score, beam, token) lists as ``beam_topk`` returns them.  True when the search is over; else
+        ``parents`` and ``next_tokens`` say how the beams go on."""
+        for score, beam, token in candidates[:self.beams]:
+            if token in self.stop:
+                self._end(score, self.tokens[beam] + [token])
+        self.parents = [beam for _, beam, _ in live]
+        self.next_tokens = [max(token, 0) for _, _, token in live]          # beams that are gone run along with any token
+        self.tokens = [self.tokens[beam] + [token] if beam >= 0 else [] for _, beam, token in live]
+        self.scores = [score for score, _, _ in live]
+        best = max(self.scores)
+        n = max(len(t) for t in self.tokens)
+        if best > -math.inf and n >= self.max_new_tokens:
+            for score, tokens in zip(self.scores, self.tokens):
+                if score > -math.inf:
+                    self._end(score, tokens)
+            return True
+        return best == -math.inf or (len(self.ended) == self.beams and self.ended[-1][0] >= self._rate(best, n))
+
+    @property
+    def choices(self) -> int:
+        """Continuations to ask for: enough for ``beams`` that do not end, if ``beam_topk`` gives that many."""
+        return min(K.BEAM_MAX_K, self.beams * (1 + len(self.stop)))
+
+
+def advance(logits: torch.Tensor, searches: Sequence[Tuple[BeamSearch, Sequence[int]]]) -> List[bool]:
+    """Lets every search choose from its rows of ``logits`` (one row after the prompt, one per beam later); True where it is over."""
+    groups: Dict[tuple, list] = {}
+    for i, (s, _) in enumerate(searches):
+        groups.setdefault((s.beams, s.stop, s.choices), []).append(i)
+    over: List[Optional[bool]] = [None] * len(searches)
+    for (beams, stop, k), members in groups.items():
+        rows = [r for i in members for r in (list(searches[i][1]) * beams)[:beams]]
+        if rows == list(range(rows[0], rows[0] + len(rows))):
+            x = logits[rows[0]:rows[0] + len(rows)]
+        elif len(members) == 1:
+            x = logits[rows[0]:rows[0] + 1].expand(beams, -1)
+        else:
+            x = logits[torch.tensor(rows, device=logits.device)]
+        scores = torch.tensor([searches[i][0].scores for i in members], dtype=torch.float32).to(logits.device)
+        out = K.beam_topk(x, scores, min(k, beams * x.shape[1]), torch.tensor(stop, dtype=torch.int32, device=logits.device))
+        flat = torch.cat([t.view(torch.int32) for t in out], dim=1).cpu()          # one copy to the host
+        parts = flat.split([t.shape[1] for t in out], dim=1)
+        lists = [p.contiguous().view(torch.float32).tolist() if j % 3 == 0 else p.tolist() for j, p in enumerate(parts)]
+        for n, i in enumerate(members):
+            over[i] = searches[i][0].update(list(zip(*(p[n] for p in lists[:3]))), list(zip(*(p[n] for p in lists[3:]))))
+    return over

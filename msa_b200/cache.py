@@ -138,6 +138,7 @@ class SequenceStateCache(SparseCache):
         self._free: List[int] = list(range(n_slots - 1, -1, -1))
         self._slot: Dict[Hashable, int] = {}
         self._length: Dict[Hashable, int] = {}
+        self._shared: Dict[Tuple[Hashable, ...], List[List[int]]] = {}
         self._parts: Optional[torch.Tensor] = None
         if self.device.type == "cuda":
             self._state_parts()              # here, so that a first ``reorder`` may be captured
@@ -160,6 +161,8 @@ class SequenceStateCache(SparseCache):
     def release(self, seq: Hashable) -> None:
         self._free.append(self._slot.pop(seq))
         del self._length[seq]
+        for group in [g for g in self._shared if seq in g]:
+            del self._shared[group]
 
     def slot(self, seq: Hashable) -> int:
         return self._slot[seq]
@@ -224,6 +227,52 @@ class SequenceStateCache(SparseCache):
                 A.call("msa_lm_reorder", A.ptr(slot), A.ptr(parent), A.ptr(length), A.ptr(shared), batch, beams, self.n_slots, A.ptr(parts),
                        parts.shape[0], A.ptr(slot_out), A.ptr(shared_out), A.ptr(work), A.stream_ptr(slot.device))
         return slot_out, shared_out
+
+    def reorder_beams(self, groups: Sequence[Sequence[Hashable]], parents: Sequence[Sequence[int]]) -> None:
+        """``reorder`` by sequence: ``groups[q]`` are the sequences of question q's beams (as many for every question), and beam j goes on from
+        beam ``parents[q][j]``, or from nobody (-1).  Beams that others go on from hold equally many positions; afterwards all of the
+        question do, and ``slot`` and ``length`` say where and how many.  One copy of tables to the device, no read-back."""
+        groups, parents = [tuple(g) for g in groups], [list(p) for p in parents]
+        if not groups:
+            return
+        beams = len(groups[0])
+        if len(parents) != len(groups) or any(len(g) != beams for g in groups) or any(len(p) != beams for p in parents) or not 1 <= beams <= 32:
+            raise ValueError("reorder_beams: groups of 1 to 32 sequences, all of one size, with a parent for each")
+        seqs = [s for g in groups for s in g]
+        if len(set(seqs)) != len(seqs) or any(s not in self._slot for s in seqs):
+            raise ValueError("reorder_beams: a sequence appears twice or holds no slot")
+        slots, lengths, tables, new = [], [], [], []
+        for g, p in zip(groups, parents):
+            if any(not -1 <= x < beams for x in p):
+                raise ValueError(f"reorder_beams: parents {p} of {beams} beams")
+            held = {self._length[g[x]] for x in p if x >= 0}
+            if len(held) > 1:
+                raise ValueError(f"reorder_beams: beams of {sorted(held)} positions cannot go on together")
+            n = held.pop() if held else 0
+            named, taken, own = set(p), set(), []
+            spare = [i for i in range(beams) if i not in named]
+            for x in p:                                             # what the kernel does with the slots
+                own.append(x if x >= 0 and x not in taken else spare.pop(0))
+                taken.add(x)
+            start = self._shared.get(g) or [[0] * beams for _ in range(beams)]
+            origin = [x if x >= 0 else o for x, o in zip(p, own)]
+            table = [[n if a == b else start[a][b] for b in origin] for a in origin]
+            slots.append([self._slot[s] for s in g])
+            lengths.append(n)
+            tables.append(start)
+            new.append((own, n, table))
+        if any(x != j for p in parents for j, x in enumerate(p)):   # else nobody moves
+            flat = torch.tensor([x for t in (slots, parents) for row in t for x in row] + lengths + [x for t in tables for row in t for x in row],
+                                dtype=torch.int32)
+            if self.device.type == "cuda":
+                flat = flat.pin_memory()
+            flat, b = flat.to(self.device, non_blocking=True), len(groups)
+            slot, parent, length, shared = flat.split([b * beams, b * beams, b, b * beams * beams])
+            self.reorder(slot.view(b, beams), parent.view(b, beams), length, shared.view(b, beams, beams))
+        for g, held, (own, n, table) in zip(groups, slots, new):
+            for s, o in zip(g, own):
+                self._slot[s], self._length[s] = held[o], n
+            self._shared[g] = table
 
     def state_bytes(self) -> int:
         return sum(t.numel() * t.element_size() for d in (self.ring, self.state, self.conv, self.shift) for t in d.values())

@@ -67,6 +67,8 @@ class GenerateConfig:
     state_slots: int = 64         # sequences in flight per GPU
     max_context: int = 8192       # prompt and generated tokens of one sequence
     seed: Optional[int] = None    # sampling: row i of a request draws from seed + i
+    num_beams: int = 1            # more than one: beam search (a state slot per beam), the best result is returned
+    length_penalty: float = 1.0   # results are rated by score / tokens ** length_penalty
 
     def __post_init__(self):
         if isinstance(self.template, str):
@@ -171,6 +173,8 @@ class MSAEngine:
         self.world_size = generate_config.world
         self.generate_config, self.model_config, self.memory_config = generate_config, model_config, memory_config
         self.serves = _serves(model_config.model_path)
+        if generate_config.num_beams != 1 and self.serves == "memory":
+            raise ValueError("num_beams: beam search is for models on state slots")
         self._service_main = service_main or (state_service_main if self.serves == "states" else MSAEngine.service_main)
         self.tokenizer = tokenizer
         self.worker_processes: List[mp.Process] = []
@@ -553,6 +557,7 @@ def state_service_main(gpu_id: int, request_queue, response_queue, generate_conf
                     break
                 key = (cmd.msg_id, cmd.seq_id)
                 rows = [SequenceRequest(tokens=ids, max_new_tokens=generate_config.max_generate_tokens, eos_token_ids=eos,
+                                        beams=generate_config.num_beams, length_penalty=generate_config.length_penalty,
                                         temperature=generate_config.temperature, top_p=generate_config.top_p, tag=key,
                                         seed=None if generate_config.seed is None else generate_config.seed + i)
                         for i, ids in enumerate(cmd.input_ids)]

@@ -124,7 +124,7 @@ def test_entry_points_refuse():
                dict(dtype=ok, live=(p, None, p)), dict(dtype=ok, logits=None), dict(dtype=ok, batch=-1)):
         assert choice(**kw) != 0 and b"beam_topk" in lib.msa_last_error()
     assert choice(dtype=ok, batch=0) == 0
-    assert lib.msa_lm_beam_topk_workspace(0, 4, 100, 8) == 0 and lib.msa_lm_beam_topk_workspace(2, 4, 100, 8) >= 2 * 4 * (16 + 8 * 8)
+    assert lib.msa_lm_beam_topk_workspace(0, 4, 100, 8) == 0 and lib.msa_lm_beam_topk_workspace(2, 4, 100, 8) >= 2 * 4 * 16
 
     def reorder(batch=2, beams=4, n_slots=9, n_part=1, slot=p, slot_out=p + 64, shared=None, shared_out=None, work=p):
         return lib.msa_lm_reorder(slot, p, p, shared, batch, beams, n_slots, p, n_part, slot_out, shared_out, work, None)
