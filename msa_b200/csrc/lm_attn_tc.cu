@@ -27,7 +27,6 @@ constexpr float kWaRescale = 8.f;
 struct WindowAttnTcParams {
   const int32_t *start, *cu, *ctx_off;   // ctx_off counts from seq0
   int seq0, heads, window;
-  int first;                             // tokens that stay visible in front of the window
   int q_row0;                            // packed row of the first query row of the map
   int q_head, k_head, v_head;            // column strides of a head
   int group;                             // query heads per key / value head
@@ -41,14 +40,7 @@ struct WindowAttnTcParams {
 
 // Items are numbered from every portion's last row block to its first: the late ones see the most keys, and the
 // fixed-stride walk of the persistent CTAs then ends on short ones.
-// Key tiles 0 .. n_first-1 hold the context's first rows, the others start at its row `base`, the first that the window reaches (or
-// where the first rows' tiles end); query tile q takes part in the tiles below f[q] and in a[q] .. b[q]-1.
-struct WaItem {
-  int len, r0, h, q_row, k_row, old, base, n_first, n_kt, f[kWaTiles], a[kWaTiles], b[kWaTiles];
-  bool valid;
-  __device__ __forceinline__ bool has(int q, int t) const { return t < f[q] || (t >= a[q] && t < b[q]); }
-  __device__ __forceinline__ int key(int t) const { return t < n_first ? t * kWaKeys : base + (t - n_first) * kWaKeys; }   // context row of a tile's first key
-};
+struct WaItem { int len, r0, h, q_row, k_row, old, n_kt, a[kWaTiles], b[kWaTiles]; bool valid; };
 __device__ __forceinline__ WaItem wa_item(const WindowAttnTcParams& p, long long w) {
   WaItem it;
   const int x = (int)(w / p.n_sh);
@@ -60,26 +52,22 @@ __device__ __forceinline__ WaItem wa_item(const WindowAttnTcParams& p, long long
   const int n_mb = (it.len + kWaRows * kWaTiles - 1) / (kWaRows * kWaTiles);
   it.valid = x < n_mb;
   it.r0 = (n_mb - 1 - x) * kWaRows * kWaTiles;
-  it.old = old_rows(p.start[s], p.first + p.window);
+  it.old = min(p.start[s], p.window - 1);
   it.q_row = c0 - p.q_row0 + it.r0;
-  it.k_row = p.ctx_off[ps];
-  it.n_first = (p.first + kWaKeys - 1) / kWaKeys;
-  it.base = max(it.n_first * kWaKeys, it.old + it.r0 - p.window + 1);
+  const int j_lo = max(0, it.old + it.r0 - p.window + 1);
+  it.k_row = p.ctx_off[ps] + j_lo;
   it.n_kt = 0;
 #pragma unroll
   for (int q = 0; q < kWaTiles; ++q) {
     const int first = it.r0 + q * kWaRows, last = min(first + kWaRows, it.len) - 1;
-    it.f[q] = it.a[q] = it.b[q] = 0;
+    it.a[q] = it.b[q] = 0;
     if (first < it.len) {
-      const int end = it.old + last + 1;         // behind the last row's own key
-      it.f[q] = min(it.n_first, (end + kWaKeys - 1) / kWaKeys);
-      if (end > it.base) {
-        it.a[q] = it.n_first + (max(it.base, it.old + first - p.window + 1) - it.base) / kWaKeys;
-        it.b[q] = it.n_first + (end - it.base + kWaKeys - 1) / kWaKeys;
-      }
-      it.n_kt = max(it.n_kt, max(it.f[q], it.b[q]));
+      it.a[q] = (max(0, it.old + first - p.window + 1) - j_lo) / kWaKeys;
+      it.b[q] = (it.old + last - j_lo) / kWaKeys + 1;
+      it.n_kt = max(it.n_kt, it.b[q]);
     }
   }
+  it.old -= j_lo;      // from here on: context index of row r relative to the item's first key = old + r
   return it;
 }
 
@@ -148,7 +136,7 @@ window_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_c
         for (int t = 0; t < it.n_kt; ++t, ++n_t) {
           const uint32_t st = n_t & 1u, ph = (n_t >> 1) & 1u;
           unsigned char* ks = kv_smem + st * kStage;
-          const int y = it.k_row + it.key(t);
+          const int y = it.k_row + t * kWaKeys;
           if (!(ok = mbar_wait(&s_k_empty[st], ph ^ 1u, abort_flag, p.status, 1))) break;
           mbar_expect_tx(&s_k_full[st], QB * kWaKBlk);
 #pragma unroll
@@ -202,12 +190,11 @@ window_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_c
           if (!(ok = wait_k(n_t + t))) break;
 #pragma unroll
           for (int q = 0; q < kWaTiles; ++q)
-            if (it.has(q, t)) issue_s(n_t + t, q);
+            if (t >= it.a[q] && t < it.b[q]) issue_s(n_t + t, q);
           tc_commit(&s_k_empty[(n_t + t) & 1u]);
           if (t + 1 == it.n_kt) tc_commit(&s_q_empty);
         }
         if (!ok) break;
-        uint32_t joined = 0u;                                  // query tiles whose O holds something
         for (int t = 0; t < it.n_kt; ++t, ++n_t) {
           const uint32_t st = n_t & 1u, ph = (n_t >> 1) & 1u;
           const bool more = t + 2 < it.n_kt;
@@ -216,20 +203,19 @@ window_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_c
           bool have_k = false;
 #pragma unroll
           for (int q = 0; q < kWaTiles; ++q) {
-            if (it.has(q, t)) {
+            if (t >= it.a[q] && t < it.b[q]) {
               const uint32_t pb = n_p[q] & 1u;
               if (!(ok = mbar_wait(&s_p_full[q][pb], (n_p[q] >> 1) & 1u, abort_flag, p.status, 4))) break;
               tc_fence_after();
 #pragma unroll
               for (int j = 0; j < kWaKeys / 16; ++j)
                 tc_mma_bf16_ts(tmem_base + kColO + (uint32_t)(q * VB * 64), tmem_base + (uint32_t)(q * 2 * kWaKeys) + pb * kWaKeys + (uint32_t)(8 * j),
-                               make_smem_desc_mn(va + j * 2048, kWaKBlk), idesc_pv, ((joined >> q) & 1u) || j > 0 ? 1u : 0u);
-              joined |= 1u << q;
+                               make_smem_desc_mn(va + j * 2048, kWaKBlk), idesc_pv, (t > it.a[q] || j > 0) ? 1u : 0u);
               tc_commit(&s_o_full[q][pb]);
               ++n_p[q];
             }
             if (q + 1 == kWaTiles) tc_commit(&s_v_empty[st]);
-            if (more && it.has(q, t + 2)) {   // in order behind the PV that read this S buffer
+            if (more && t + 2 >= it.a[q] && t + 2 < it.b[q]) {   // in order behind the PV that read this S buffer
               if (!have_k && !(ok = wait_k(n_t + 2))) break;
               have_k = true;
               issue_s(n_t + 2, q);
@@ -256,12 +242,10 @@ window_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_c
     bool ok = true;
     for (long long w = blockIdx.x; w < p.n_items && ok; w += gridDim.x) {
       const WaItem it = wa_item(p, w);
-      if (!it.valid || it.r0 + q * kWaRows >= it.len) continue;
+      if (!it.valid || it.a[q] == it.b[q]) continue;
       float m_ref = p.sink ? 0.f : -1e30f, l_run = p.sink ? 1.f : 0.f;
       const int row0 = it.r0 + q * kWaRows + wq * 32;          // first row of this warp
-      bool joined = false;                                     // O holds something of this item
-      for (int t = 0; t < max(it.f[q], it.b[q]); ++t) {
-        if (!it.has(q, t)) continue;
+      for (int t = it.a[q]; t < it.b[q]; ++t, ++n_c) {
         const uint32_t sb = n_c & 1u;
         ok = mbar_wait(&s_s_full[q][sb], (n_c >> 1) & 1u, abort_flag, p.status, 5);
         ok = __all_sync(0xffffffffu, ok);
@@ -273,20 +257,19 @@ window_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_c
         tmem_ld32(s_addr + 32, vb);
         // Key i of a chunk is visible to lane r iff r + d - window < i <= r + d, d = (index of the warp's first row) -
         // (index of the chunk's first key).
-        const int key0 = it.key(t), d0 = it.old + row0 - key0;
+        const int d0 = it.old + row0 - t * kWaKeys;
         tmem_ld_wait();
         int cls[2];
-        // n: keys of the chunk that stay visible behind the window as well.
-        auto cut = [&](uint32_t (&v)[32], int d, int n, int& c) {
-          if (d + 31 < 0 || (d - p.window >= 31 && n <= 0)) { c = 0; return; }
+        auto cut = [&](uint32_t (&v)[32], int d, int& c) {
+          if (d + 31 < 0 || d - p.window >= 31) { c = 0; return; }
           c = 2;
-          if (d >= 31 && (d + 31 - p.window < 0 || n >= 32)) return;
+          if (d >= 31 && d + 31 - p.window < 0) return;
           const int hi = lane + d, lo = lane + d - p.window;
 #pragma unroll
-          for (int i = 0; i < 32; ++i) if (i > hi || (i <= lo && i >= n)) v[i] = 0xff800000u;
+          for (int i = 0; i < 32; ++i) if (i > hi || i <= lo) v[i] = 0xff800000u;
         };
-        cut(va, d0, p.first - key0, cls[0]);
-        cut(vb, d0 - 32, p.first - key0 - 32, cls[1]);
+        cut(va, d0, cls[0]);
+        cut(vb, d0 - 32, cls[1]);
         float mx = -INFINITY, mx2 = -INFINITY;
         if (cls[0]) {
 #pragma unroll
@@ -306,7 +289,7 @@ window_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_c
         const bool move = (mx - m_ref) * p.scale_log2e > kWaRescale;
         if (__any_sync(0xffffffffu, move)) {
           const float f = move ? exp2f((m_ref - mx) * p.scale_log2e) : 1.f;
-          if (joined) {        // wait for the PV in flight, then rescale this warp's rows of O in place
+          if (t > it.a[q]) {   // wait for the PV in flight, then rescale this warp's rows of O in place
             ok = mbar_wait(&s_o_full[q][(n_c - 1u) & 1u], ((n_c - 1u) >> 1) & 1u, abort_flag, p.status, 6);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
@@ -360,8 +343,6 @@ window_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_c
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&s_p_full[q][sb]);
-        joined = true;
-        ++n_c;
       }
       if (!ok) break;
       ok = mbar_wait(&s_o_full[q][(n_c - 1u) & 1u], ((n_c - 1u) >> 1) & 1u, abort_flag, p.status, 6);
@@ -442,13 +423,14 @@ extern "C" int msa_lm_window_attn_tc_first(const msa_lm_attn_args* args, int32_t
   MSA_REQUIRE(a.dtype == MSA_BF16 && a.qa_dtype == MSA_BF16 && a.out_dtype == MSA_BF16, "window_attn_tc: bf16 only");
   MSA_REQUIRE(msa_lm_window_attn_tc_supported(dim, rot, vdim), "window_attn_tc: unsupported head sizes (%d, %d, %d)", dim, rot, vdim);
   MSA_REQUIRE(a.heads > 0 && a.window > 0 && a.scale > 0.f && a.group > 0 && a.heads % a.group == 0, "window_attn_tc: bad sizes");
-  MSA_REQUIRE(first_fits(first, a.window, 0), "window_attn_tc: bad number of first tokens");
+  MSA_REQUIRE(first == 0 || (first > 0 && rot == 0 && first <= 0x7ffffff0 - a.window), "window_attn_tc: first tokens with a rotated part, or too many of them");
   MSA_REQUIRE(rot == 0 || (a.kb && a.kb_head == 0 && a.qb == (const __nv_bfloat16*)a.qa + dim && a.qb_head == a.qa_head),
               "window_attn_tc: the rotated parts must follow the plain query part and be shared by the keys");
   MSA_REQUIRE(aligned16(a.qa) && aligned16(a.ka) && aligned16(a.v) && aligned16(a.out) && (rot == 0 || aligned16(a.kb)) &&
                   a.qa_row % 8 == 0 && a.ka_row % 8 == 0 && a.v_row % 8 == 0 && a.out_row % 8 == 0 && a.kb_row % 8 == 0 &&
                   a.qa_head % 8 == 0 && a.ka_head % 8 == 0 && a.v_head % 8 == 0 && a.out_head == vdim, "window_attn_tc: rows must be 16-byte aligned");
   if (a.seq1 <= a.seq0 || a.max_len <= 0 || n_rows <= 0) return MSA_OK;
+  if (first > 0) return first_attn_tc(a, first, n_rows, n_ctx, row0, status, (cudaStream_t)stream);
   const int kv_heads = a.heads / a.group;
   CUtensorMap mq, mk, mr, mv;
   MSA_OK_OR_RETURN(make_map(&mq, a.qa, n_rows, (uint64_t)(a.heads - 1) * a.qa_head + dim + rot, a.qa_row, 64, kWaRows));
@@ -458,7 +440,7 @@ extern "C" int msa_lm_window_attn_tc_first(const msa_lm_attn_args* args, int32_t
   else mr = mk;
   WindowAttnTcParams p{};
   p.start = a.start; p.cu = a.cu; p.ctx_off = a.ctx_off;
-  p.seq0 = a.seq0; p.heads = a.heads; p.window = a.window; p.first = first; p.q_row0 = row0;
+  p.seq0 = a.seq0; p.heads = a.heads; p.window = a.window; p.q_row0 = row0;
   p.q_head = (int)a.qa_head; p.k_head = (int)a.ka_head; p.v_head = (int)a.v_head;
   p.group = a.group; p.sink = a.sink; p.gate = (const __nv_bfloat16*)a.gate; p.gate_row = a.gate_row;
   p.scale_log2e = a.scale * 1.4426950408889634f;

@@ -7,6 +7,8 @@
 
 namespace msa {
 
+int first_attn_tc(const msa_lm_attn_args& a, int first, int n_rows, int n_ctx, int row0, int32_t* status, cudaStream_t stream);   // lm_first_tc.cu
+
 template <typename T> __device__ __forceinline__ float to_f(T v);
 template <> __device__ __forceinline__ float to_f<float>(float v) { return v; }
 template <> __device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
