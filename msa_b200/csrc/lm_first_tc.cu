@@ -8,7 +8,8 @@
 // keys lie outside a row's window.  One persistent CTA per SM, 320 threads: warps 0-3 the softmax of tile 0, 4-7 that of tile 1 (thread =
 // row = TMEM lane), warp 8 the TMA producer, warp 9 the MMA issuer.  Per 128 keys and row tile:
 //     S = Q K^T    fp32 into the tile's 128 TMEM columns;
-//     softmax      fp32, running maximum advanced only when it moved by more than 2^8; P as bf16 over the consumed columns, in halves;
+//     softmax      fp32; the reference moves only when the maximum is 2^32 above it (fp32 sums and bf16 weights keep their relative
+//                  precision up to there, and O is rescaled all but never); P as bf16 over the consumed columns, in halves;
 //     O += P V     A = P from TMEM, B = V MN-major; O stays in TMEM.
 // While one tile's softmax runs, the tensor pipe works for the other.  128 keys because an issued product takes some 70 cycles
 // whatever its columns: with 64 the issuing thread was the bound (3460 cycles for 64 keys of both tiles, 2200 of them issuing).
@@ -25,7 +26,7 @@ constexpr int kFtThreads = 32 * (4 * kFtTiles + 2);
 constexpr int kFtBlk = kFtRows * 128;                     // one 64-column block of a row, key or value tile: 16 KB
 constexpr int kFtStage = 32 * 64;                         // per softmax warp: 32 rows x 32 bf16 of output
 constexpr uint32_t kFtTmem = 512, kFtColO = kFtTiles * kFtKeys;
-constexpr float kFtRescale = 8.f;
+constexpr float kFtRescale = 32.f;
 
 struct FirstAttnParams {
   const int32_t *start, *cu, *ctx_off;   // ctx_off counts from seq0
@@ -275,21 +276,11 @@ first_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + 32 * c, v[c]);
         tmem_ld_wait();
-        int cls[4];                                           // a chunk of 32 slots: 0 hidden, 2 visible in part or whole
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        const int s_tile = t * kFtKeys, k_tile = s_tile + it.shift - it.old;       // first slot, and its token if none are first rows
+        if (s_tile < p.pad || k_tile + kFtKeys - 1 > row0 || k_tile <= row1 - p.window) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int s0 = t * kFtKeys + 32 * c;
-          bool all;
-          if (s0 >= p.pad) {                                  // key row = slot + shift
-            const int k0 = s0 + it.shift - it.old;
-            cls[c] = k0 > row1 || k0 + 31 <= row0 - p.window ? 0 : 2;
-            all = k0 + 31 <= row0 && k0 > row1 - p.window;
-          } else {
-            cls[c] = s0 - it.old > row1 ? 0 : 2;
-            all = s0 + 31 < p.first && s0 + 31 - it.old <= row0;
-          }
-          if (cls[c] && !all) {
+          for (int c = 0; c < 4; ++c) {
+            const int s0 = s_tile + 32 * c;
             uint32_t seen = slot_bits(mine - p.window - it.shift, mine - it.shift, s0);
             if (s0 < p.pad) {
               const uint32_t front = slot_bits(s0 - 1, p.pad - 1, s0);
@@ -298,17 +289,20 @@ first_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
 #pragma unroll
             for (int i = 0; i < 32; ++i) if (!((seen >> i) & 1u)) v[c][i] = 0xff800000u;
           }
-          if (cls[c]) {
-            float m2 = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              mx[c] = max3(mx[c], __uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1]));
-              m2 = max3(m2, __uint_as_float(v[c][i + 2]), __uint_as_float(v[c][i + 3]));
-            }
-            mx[c] = fmaxf(mx[c], m2);
-          }
         }
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        float mx[8];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          mx[2 * c] = __uint_as_float(v[c][0]);
+          mx[2 * c + 1] = __uint_as_float(v[c][1]);
+#pragma unroll
+          for (int i = 2; i < 30; i += 4) {
+            mx[2 * c] = max3(mx[2 * c], __uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1]));
+            mx[2 * c + 1] = max3(mx[2 * c + 1], __uint_as_float(v[c][i + 2]), __uint_as_float(v[c][i + 3]));
+          }
+          mx[2 * c] = max3(mx[2 * c], __uint_as_float(v[c][30]), __uint_as_float(v[c][31]));
+        }
+        const float top = max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7]));
         const bool move = (top - m_ref) * p.scale_log2e > kFtRescale;
         if (__any_sync(0xffffffffu, move)) {
           const float f = move ? exp2f((m_ref - top) * p.scale_log2e) : 1.f;
@@ -336,21 +330,16 @@ first_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           uint32_t pk[16];
-          if (cls[c] == 0) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) pk[i] = 0u;
-          } else {
-#pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              float x0, x1, x2, x3;
-              f32x2_split(fma_f32x2(f32x2(__uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1])), scale2, neg_m2), x0, x1);
-              f32x2_split(fma_f32x2(f32x2(__uint_as_float(v[c][i + 2]), __uint_as_float(v[c][i + 3])), scale2, neg_m2), x2, x3);
-              const float e0 = ex2_approx(x0), e1 = ex2_approx(x1), e2 = ex2_approx(x2), e3 = ex2_approx(x3);
-              sum_a = add_f32x2(sum_a, f32x2(e0, e1));
-              sum_b = add_f32x2(sum_b, f32x2(e2, e3));
-              pk[i >> 1] = pack2_bf16(e0, e1);
-              pk[(i >> 1) + 1] = pack2_bf16(e2, e3);
-            }
+          for (int i = 0; i < 32; i += 4) {
+            float x0, x1, x2, x3;
+            f32x2_split(fma_f32x2(f32x2(__uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1])), scale2, neg_m2), x0, x1);
+            f32x2_split(fma_f32x2(f32x2(__uint_as_float(v[c][i + 2]), __uint_as_float(v[c][i + 3])), scale2, neg_m2), x2, x3);
+            const float e0 = ex2_approx(x0), e1 = ex2_approx(x1), e2 = ex2_approx(x2), e3 = ex2_approx(x3);
+            sum_a = add_f32x2(sum_a, f32x2(e0, e1));
+            sum_b = add_f32x2(sum_b, f32x2(e2, e3));
+            pk[i >> 1] = pack2_bf16(e0, e1);
+            pk[(i >> 1) + 1] = pack2_bf16(e2, e3);
           }
           tmem_st16(s_addr + 16 * c, pk);
           if (c & 1) {                                        // half of P is there
