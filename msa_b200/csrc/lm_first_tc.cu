@@ -9,10 +9,12 @@
 // row = TMEM lane), warp 8 the TMA producer, warp 9 the MMA issuer.  Per 128 keys and row tile:
 //     S = Q K^T    fp32 into the tile's 128 TMEM columns;
 //     softmax      fp32; the reference moves only when the maximum is 2^32 above it (fp32 sums and bf16 weights keep their relative
-//                  precision up to there, and O is rescaled all but never); P as bf16 over the consumed columns, in halves;
+//                  precision up to there, and O is rescaled all but never); P as bf16 over the consumed columns;
 //     O += P V     A = P from TMEM, B = V MN-major; O stays in TMEM.
 // While one tile's softmax runs, the tensor pipe works for the other.  128 keys because an issued product takes some 70 cycles
-// whatever its columns: with 64 the issuing thread was the bound (3460 cycles for 64 keys of both tiles, 2200 of them issuing).
+// whatever its columns: with 64 the issuing thread was the bound (3460 cycles for 64 keys of both tiles, 2200 of them issuing).  That
+// thread is kept to one wait for copies, two for P and three commits per 128 keys: each costs it 90 to 140 cycles (4130 cycles an
+// iteration with six of each).  Two issuing threads are slower (368 us where one takes 298).
 //
 // Keys come as slots: the context's first rows up to a multiple of 8, then its rows from `base` on, the first that the item's window
 // reaches (or where those rows end).  A tile in which the two meet is fetched by two copies, so that few first tokens cost no tile.
@@ -24,7 +26,7 @@ namespace msa {
 constexpr int kFtRows = 128, kFtTiles = 2, kFtKeys = 128;
 constexpr int kFtThreads = 32 * (4 * kFtTiles + 2);
 constexpr int kFtBlk = kFtRows * 128;                     // one 64-column block of a row, key or value tile: 16 KB
-constexpr int kFtStage = 32 * 64;                         // per softmax warp: 32 rows x 32 bf16 of output
+constexpr int kFtKeyBufs = 3;
 constexpr uint32_t kFtTmem = 512, kFtColO = kFtTiles * kFtKeys;
 constexpr float kFtRescale = 32.f;
 
@@ -94,8 +96,8 @@ first_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
                      const __grid_constant__ CUtensorMap tmap_v1, const FirstAttnParams p) {
   static_assert(kFtColO + kFtTiles * VB * 64 <= kFtTmem, "TMEM columns");
   extern __shared__ unsigned char smem_dyn[];
-  __shared__ uint64_t s_q_full, s_q_empty, s_k_full[2], s_k_empty[2], s_v_full[2], s_v_empty[2], s_drain;
-  __shared__ uint64_t s_s_full[kFtTiles], s_p_full[kFtTiles][2], s_o_full[kFtTiles];
+  __shared__ uint64_t s_q_full, s_q_empty, s_kv_full[2], s_kv_empty[2], s_drain;
+  __shared__ uint64_t s_s_full[kFtTiles], s_p_full[kFtTiles], s_o_full[kFtTiles];
   __shared__ uint32_t s_tmem_base;
   __shared__ int s_abort;
 
@@ -103,19 +105,14 @@ first_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
   unsigned char* tiles = reinterpret_cast<unsigned char*>(((uintptr_t)smem_dyn + 1023) & ~(uintptr_t)1023);
   unsigned char* q_smem = tiles;
   unsigned char* k_smem = q_smem + kFtTiles * DB * kFtBlk;
-  unsigned char* v_smem = k_smem + 2 * DB * kFtBlk;
-  unsigned char* out_stage = v_smem + 2 * VB * kFtBlk;
+  unsigned char* v_smem = k_smem + kFtKeyBufs * DB * kFtBlk;
   volatile int* abort_flag = &s_abort;
 
   if (threadIdx.x == 0) {
     mbar_init(&s_q_full, 1); mbar_init(&s_q_empty, 1); mbar_init(&s_drain, 1);
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&s_k_full[i], 1); mbar_init(&s_k_empty[i], 1);
-      mbar_init(&s_v_full[i], 1); mbar_init(&s_v_empty[i], 1);
-    }
+    for (int i = 0; i < 2; ++i) { mbar_init(&s_kv_full[i], 1); mbar_init(&s_kv_empty[i], 1); }
     for (int q = 0; q < kFtTiles; ++q) {
-      mbar_init(&s_s_full[q], 1); mbar_init(&s_o_full[q], 1);
-      mbar_init(&s_p_full[q][0], 4); mbar_init(&s_p_full[q][1], 4);
+      mbar_init(&s_s_full[q], 1); mbar_init(&s_p_full[q], 4); mbar_init(&s_o_full[q], 1);
     }
     s_abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -130,12 +127,16 @@ first_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
   tc_fence_after();
   const uint32_t tmem_base = s_tmem_base;
 
-  // Every role walks the same items.  n_t counts the CTA's key tiles (stage and phase of the K / V barriers), n_c[q] the tiles that row
-  // tile q took part in (phase of its S / P / O barriers), n_it the items (the query buffer).
+  // Every role walks the same items.  Keys come one tile ahead of their values: an item starts with its queries and first keys, and turn t
+  // brings the values of tile t with the keys of tile t + 1.  n_t counts the turns (stage and phase of the K / V barriers), n_c the tiles
+  // that a row tile took part in (phase of its S and P barriers), n_o its items, n_it all items.  Turn n_t waits for the end of turn n_t - 2,
+  // in front of which S of an item's first keys may not have been issued: three buffers of keys, taken in turn (b_k), so that
+  // those are overwritten two turns after S's own.
   if (warp == 4 * kFtTiles) {
     if (lane == 0) {
-      uint32_t n_it = 0, n_t = 0;
+      uint32_t n_it = 0, n_t = 0, b_k = 0;
       bool ok = true;
+      auto next = [](uint32_t b) { return b + 1 == kFtKeyBufs ? 0u : b + 1; };
       // One key or value tile: slots 128 t .. of `heads` columns from x on.
       auto load = [&](unsigned char* dst, const CUtensorMap* full, const CUtensorMap* front, const CUtensorMap* back, int blocks, int x, const FtItem& it, int t,
                       uint64_t* bar) {
@@ -154,20 +155,25 @@ first_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         const FtItem it = ft_item(p, w);
         if (!it.valid) continue;
         if (!(ok = mbar_wait(&s_q_empty, (n_it & 1u) ^ 1u, abort_flag, p.status, 1))) break;
-        mbar_expect_tx(&s_q_full, kFtTiles * DB * kFtBlk);
+        const int k_col = it.h / p.group * p.k_head, v_col = it.h / p.group * p.v_head;
+        mbar_expect_tx(&s_q_full, (kFtTiles + 1) * DB * kFtBlk);
 #pragma unroll
         for (int q = 0; q < kFtTiles; ++q)
 #pragma unroll
           for (int c = 0; c < DB; ++c)
             tma_load_3d(q_smem + (q * DB + c) * kFtBlk, &tmap_q, 64 * c, it.h, it.q_row + q * (kFtRows >> p.pack), &s_q_full);
+        load(k_smem + b_k * DB * kFtBlk, &tmap_k, &tmap_k0, &tmap_k1, DB, k_col, it, 0, &s_q_full);
+        b_k = next(b_k);
         for (int t = 0; t < it.n_kt; ++t, ++n_t) {
           const uint32_t st = n_t & 1u, ph = (n_t >> 1) & 1u;
-          if (!(ok = mbar_wait(&s_k_empty[st], ph ^ 1u, abort_flag, p.status, 1))) break;
-          mbar_expect_tx(&s_k_full[st], DB * kFtBlk);
-          load(k_smem + st * DB * kFtBlk, &tmap_k, &tmap_k0, &tmap_k1, DB, it.h / p.group * p.k_head, it, t, &s_k_full[st]);
-          if (!(ok = mbar_wait(&s_v_empty[st], ph ^ 1u, abort_flag, p.status, 1))) break;
-          mbar_expect_tx(&s_v_full[st], VB * kFtBlk);
-          load(v_smem + st * VB * kFtBlk, &tmap_v, &tmap_v0, &tmap_v1, VB, it.h / p.group * p.v_head, it, t, &s_v_full[st]);
+          const bool more = t + 1 < it.n_kt;
+          if (!(ok = mbar_wait(&s_kv_empty[st], ph ^ 1u, abort_flag, p.status, 1))) break;
+          mbar_expect_tx(&s_kv_full[st], (VB + (more ? DB : 0)) * kFtBlk);
+          load(v_smem + st * VB * kFtBlk, &tmap_v, &tmap_v0, &tmap_v1, VB, v_col, it, t, &s_kv_full[st]);
+          if (more) {
+            load(k_smem + b_k * DB * kFtBlk, &tmap_k, &tmap_k0, &tmap_k1, DB, k_col, it, t + 1, &s_kv_full[st]);
+            b_k = next(b_k);
+          }
         }
         ++n_it;
       }
@@ -181,70 +187,53 @@ first_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       const uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kFtKeys >> 3) << 17) | ((uint32_t)(kFtRows >> 4) << 24);
       const uint32_t idesc_pv = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(VB * 64 >> 3) << 17) |
                                 ((uint32_t)(kFtRows >> 4) << 24);
-      const uint32_t qa = smem_u32(q_smem), ka = smem_u32(k_smem), va = smem_u32(v_smem);
-      uint32_t n_it = 0, n_t = 0, n_p[kFtTiles] = {};        // n_p: PV tiles issued so far
+      const uint64_t q_desc = make_smem_desc(smem_u32(q_smem)), k_desc = make_smem_desc(smem_u32(k_smem)),
+                     v_desc = make_smem_desc_mn(smem_u32(v_smem), kFtBlk);
+      uint32_t n_it = 0, n_t = 0, b_k = 0, n_p[kFtTiles] = {};   // n_p: PV tiles issued so far
       bool ok = true;
-      auto issue_s = [&](uint32_t g, int q) {                // S of the CTA's key tile g for row tile q
+      auto issue_s = [&](uint32_t g, int q) {                // S of the keys in buffer g for row tile q
+        const uint64_t b_desc = k_desc + (uint64_t)(g * (DB * kFtBlk >> 4));
 #pragma unroll
-        for (int c = 0; c < DB; ++c) {
-          const uint64_t a_desc = make_smem_desc(qa + (q * DB + c) * kFtBlk), b_desc = make_smem_desc(ka + ((g & 1u) * DB + c) * kFtBlk);
+        for (int c = 0; c < DB; ++c)
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            tc_mma_bf16(tmem_base + (uint32_t)(q * kFtKeys), a_desc + (uint64_t)(2 * k), b_desc + (uint64_t)(2 * k), idesc_s, (c > 0 || k > 0) ? 1u : 0u);
-        }
+            tc_mma_bf16(tmem_base + (uint32_t)(q * kFtKeys), q_desc + (uint64_t)(((q * DB + c) * kFtBlk >> 4) + 2 * k),
+                        b_desc + (uint64_t)((c * kFtBlk >> 4) + 2 * k), idesc_s, (c > 0 || k > 0) ? 1u : 0u);
         tc_commit(&s_s_full[q]);
-      };
-      auto wait_k = [&](uint32_t g) {
-        const bool r = mbar_wait(&s_k_full[g & 1u], (g >> 1) & 1u, abort_flag, p.status, 3);
-        tc_fence_after();
-        return r;
       };
       for (long long w = blockIdx.x; w < p.n_items && ok; w += gridDim.x) {
         const FtItem it = ft_item(p, w);
         if (!it.valid) continue;
         if (!(ok = mbar_wait(&s_q_full, n_it & 1u, abort_flag, p.status, 2))) break;
-        if (!(ok = wait_k(n_t))) break;
+        tc_fence_after();
 #pragma unroll
         for (int q = 0; q < kFtTiles; ++q)
-          if (it.has(q, 0)) issue_s(n_t, q);                  // behind the last item's products that read these columns
-        tc_commit(&s_k_empty[n_t & 1u]);
+          if (it.has(q, 0)) issue_s(b_k, q);                  // behind the last item's products that read these columns
+        b_k = b_k + 1 == kFtKeyBufs ? 0u : b_k + 1;
         if (it.n_kt == 1) tc_commit(&s_q_empty);
-        uint32_t joined = 0u;                                 // row tiles whose O holds something
         for (int t = 0; t < it.n_kt; ++t, ++n_t) {
           const uint32_t st = n_t & 1u;
           const bool more = t + 1 < it.n_kt;
-          if (!(ok = mbar_wait(&s_v_full[st], (n_t >> 1) & 1u, abort_flag, p.status, 3))) break;
-          bool have_k = false;
+          if (!(ok = mbar_wait(&s_kv_full[st], (n_t >> 1) & 1u, abort_flag, p.status, 3))) break;
+          const uint64_t b_desc = v_desc + (uint64_t)(st * (VB * kFtBlk >> 4));
 #pragma unroll
           for (int q = 0; q < kFtTiles; ++q) {
             if (it.has(q, t)) {
+              if (!(ok = mbar_wait(&s_p_full[q], n_p[q] & 1u, abort_flag, p.status, 4))) break;
+              tc_fence_after();
 #pragma unroll
-              for (int half = 0; half < 2; ++half) {
-                if (!(ok = mbar_wait(&s_p_full[q][half], n_p[q] & 1u, abort_flag, p.status, 4))) break;
-                tc_fence_after();
-#pragma unroll
-                for (int j = half * 4; j < half * 4 + 4; ++j)
-                  tc_mma_bf16_ts(tmem_base + kFtColO + (uint32_t)(q * VB * 64), tmem_base + (uint32_t)(q * kFtKeys + 8 * j),
-                                 make_smem_desc_mn(va + st * VB * kFtBlk + j * 2048, kFtBlk), idesc_pv, ((joined >> q) & 1u) || j > 0 ? 1u : 0u);
-              }
-              if (!ok) break;
-              joined |= 1u << q;
-              tc_commit(&s_o_full[q]);
+              for (int j = 0; j < kFtKeys / 16; ++j)
+                tc_mma_bf16_ts(tmem_base + kFtColO + (uint32_t)(q * VB * 64), tmem_base + (uint32_t)(q * kFtKeys + 8 * j), b_desc + (uint64_t)(j * (2048 >> 4)),
+                               idesc_pv, t > 0 || j > 0 ? 1u : 0u);
+              if (t + 1 == it.b[q]) tc_commit(&s_o_full[q]);
               ++n_p[q];
             }
-            if (q + 1 == kFtTiles) tc_commit(&s_v_empty[st]);
-            if (more && it.has(q, t + 1)) {                   // in order behind the PV that read these columns
-              if (!have_k && !(ok = wait_k(n_t + 1))) break;
-              have_k = true;
-              issue_s(n_t + 1, q);
-            }
+            if (more && it.has(q, t + 1)) issue_s(b_k, q);    // in order behind the PV that read these columns
           }
           if (!ok) break;
-          if (more) {
-            if (!have_k && !(ok = wait_k(n_t + 1))) break;
-            tc_commit(&s_k_empty[(n_t + 1) & 1u]);
-            if (t + 2 == it.n_kt) tc_commit(&s_q_empty);
-          }
+          if (more) b_k = b_k + 1 == kFtKeyBufs ? 0u : b_k + 1;
+          tc_commit(&s_kv_empty[st]);
+          if (t + 2 == it.n_kt) tc_commit(&s_q_empty);
         }
         ++n_it;
       }
@@ -256,7 +245,7 @@ first_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     const int q = warp / 4, wq = warp % 4;
     const uint32_t lane_base = tmem_base + ((uint32_t)(wq * 32) << 16);
     const uint32_t s_addr = lane_base + (uint32_t)(q * kFtKeys), o_addr = lane_base + kFtColO + (uint32_t)(q * VB * 64);
-    uint32_t n_c = 0;
+    uint32_t n_c = 0, n_o = 0;
     bool ok = true;
     for (long long w = blockIdx.x; w < p.n_items && ok; w += gridDim.x) {
       const FtItem it = ft_item(p, w);
@@ -266,8 +255,8 @@ first_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       const int row0 = t_first + ((wq * 32) >> p.pack), row1 = t_first + ((wq * 32 + 31) >> p.pack);   // this warp's tokens
       const int mine = it.old + t_first + ((wq * 32 + lane) >> p.pack);                                // context row of the lane's token
       bool joined = false;                                    // O holds something of this item
-      for (int t = 0; t < it.n_kt; ++t) {
-        if (!it.has(q, t)) continue;
+      const int f_q = q ? it.f[1] : it.f[0], a_q = q ? it.a[1] : it.a[0], b_q = q ? it.b[1] : it.b[0];
+      for (int t = 0; t < b_q; t = t + 1 < f_q || t + 1 >= a_q ? t + 1 : a_q) {
         ok = mbar_wait(&s_s_full[q], n_c & 1u, abort_flag, p.status, 5);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
@@ -306,11 +295,7 @@ first_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         const bool move = (top - m_ref) * p.scale_log2e > kFtRescale;
         if (__any_sync(0xffffffffu, move)) {
           const float f = move ? exp2f((m_ref - top) * p.scale_log2e) : 1.f;
-          if (joined) {        // wait for the PV in flight, then rescale this warp's rows of O in place
-            ok = mbar_wait(&s_o_full[q], (n_c - 1u) & 1u, abort_flag, p.status, 6);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            tc_fence_after();
+          if (joined) {        // S came behind the last PV: rescale this warp's rows of O in place
 #pragma unroll
             for (int c = 0; c < VB * 4; ++c) {
               uint32_t o[16];
@@ -342,13 +327,11 @@ first_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
             pk[(i >> 1) + 1] = pack2_bf16(e2, e3);
           }
           tmem_st16(s_addr + 16 * c, pk);
-          if (c & 1) {                                        // half of P is there
-            tmem_st_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&s_p_full[q][c >> 1]);
-          }
         }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_p_full[q]);
         float s0, s1, s2, s3;
         f32x2_split(sum_a, s0, s1);
         f32x2_split(sum_b, s2, s3);
@@ -357,7 +340,7 @@ first_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         ++n_c;
       }
       if (!ok) break;
-      ok = mbar_wait(&s_o_full[q], (n_c - 1u) & 1u, abort_flag, p.status, 6);
+      ok = mbar_wait(&s_o_full[q], n_o++ & 1u, abort_flag, p.status, 6);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
@@ -366,7 +349,9 @@ first_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       float inv = 1.f / l_run;
       if (p.gate && t_first + (r_mine >> p.pack) < it.len)
         inv *= sigmoid_f(__bfloat162float(p.gate[(long long)(r_first + (r_mine >> p.pack)) * p.gate_row + it.h + (r_mine & low)]));
-      unsigned char* stg = out_stage + warp * kFtStage;
+      // A lane writes its row: 64 bytes at a time, which L2 puts together.
+      __nv_bfloat16* dst = p.out + (long long)(r_first + (r_mine >> p.pack)) * p.out_row + (it.h + (r_mine & low)) * VB * 64;
+      const bool on = t_first + (r_mine >> p.pack) < it.len;
 #pragma unroll
       for (int c = 0; c < VB * 2; ++c) {
         uint32_t o[32];
@@ -379,17 +364,8 @@ first_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
           d.y = pack2_bf16(__uint_as_float(o[8 * i + 2]) * inv, __uint_as_float(o[8 * i + 3]) * inv);
           d.z = pack2_bf16(__uint_as_float(o[8 * i + 4]) * inv, __uint_as_float(o[8 * i + 5]) * inv);
           d.w = pack2_bf16(__uint_as_float(o[8 * i + 6]) * inv, __uint_as_float(o[8 * i + 7]) * inv);
-          *reinterpret_cast<uint4*>(stg + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) = d;
+          if (on) *reinterpret_cast<uint4*>(dst + 32 * c + 8 * i) = d;
         }
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = (lane >> 2) + 8 * i, piece = lane & 3, rr = wq * 32 + r, tok = rr >> p.pack;
-          const uint4 d = *reinterpret_cast<const uint4*>(stg + r * 64 + ((piece ^ ((r >> 1) & 3)) << 4));
-          if (t_first + tok < it.len)
-            *reinterpret_cast<uint4*>(p.out + (long long)(r_first + tok) * p.out_row + (it.h + (rr & low)) * VB * 64 + 32 * c + 8 * piece) = d;
-        }
-        __syncwarp();
       }
       tc_fence_before();
     }
@@ -403,7 +379,7 @@ first_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
 
 template <int DB, int VB>
 int launch_first_attn_tc(const CUtensorMap& q, const CUtensorMap (&k)[3], const CUtensorMap (&v)[3], const FirstAttnParams& p, cudaStream_t stream) {
-  constexpr size_t smem = (size_t)(kFtTiles * DB + 2 * DB + 2 * VB) * kFtBlk + 4 * kFtTiles * kFtStage + 1024;
+  constexpr size_t smem = (size_t)((kFtTiles + kFtKeyBufs) * DB + 2 * VB) * kFtBlk + 1024;
   static_assert(smem <= 227 * 1024, "shared memory");
   static DeviceSmem configured{};
   MSA_OK_OR_RETURN(ensure_dynamic_smem(first_attn_tc_kernel<DB, VB>, smem, configured));
