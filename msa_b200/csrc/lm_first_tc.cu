@@ -54,8 +54,9 @@ struct FtItem {
 };
 __device__ __forceinline__ FtItem ft_item(const FirstAttnParams& p, long long w) {
   FtItem it;
-  const int x = (int)(w / p.n_sh), packs = p.heads >> p.pack, span = (kFtRows * kFtTiles) >> p.pack, each = kFtRows >> p.pack;
-  const int sh = (int)(w - x * p.n_sh), ps = sh / packs, s = p.seq0 + ps;
+  const uint32_t n_sh = (uint32_t)p.n_sh;
+  const int x = (int)((uint32_t)w / n_sh), packs = p.heads >> p.pack, span = (kFtRows * kFtTiles) >> p.pack, each = kFtRows >> p.pack;
+  const int sh = (int)((uint32_t)w - (uint32_t)x * n_sh), ps = sh / packs, s = p.seq0 + ps;
   it.h = (sh - ps * packs) << p.pack;
   const int c0 = p.cu[s];
   it.len = p.cu[s + 1] - c0;
@@ -349,23 +350,35 @@ first_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       float inv = 1.f / l_run;
       if (p.gate && t_first + (r_mine >> p.pack) < it.len)
         inv *= sigmoid_f(__bfloat162float(p.gate[(long long)(r_first + (r_mine >> p.pack)) * p.gate_row + it.h + (r_mine & low)]));
-      // A lane writes its row: 64 bytes at a time, which L2 puts together.
-      __nv_bfloat16* dst = p.out + (long long)(r_first + (r_mine >> p.pack)) * p.out_row + (it.h + (r_mine & low)) * VB * 64;
-      const bool on = t_first + (r_mine >> p.pack) < it.len;
+      // Eight rows of 64 bytes a store: lanes trade the 16-byte pieces of their rows, the piece's two bits for the lane's upper two.
+      const int hi = lane >> 4, mid = (lane >> 3) & 1, piece = lane >> 3;
+      __nv_bfloat16* dst[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = wq * 32 + 8 * i + (lane & 7), tok = r >> p.pack;
+        dst[i] = t_first + tok < it.len ? p.out + (long long)(r_first + tok) * p.out_row + (it.h + (r & low)) * VB * 64 + 8 * piece : nullptr;
+      }
 #pragma unroll
       for (int c = 0; c < VB * 2; ++c) {
-        uint32_t o[32];
+        uint32_t o[32], d[16];                                // d: [piece][word]
         tmem_ld32(o_addr + 32 * c, o);
         tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint4 d;
-          d.x = pack2_bf16(__uint_as_float(o[8 * i]) * inv, __uint_as_float(o[8 * i + 1]) * inv);
-          d.y = pack2_bf16(__uint_as_float(o[8 * i + 2]) * inv, __uint_as_float(o[8 * i + 3]) * inv);
-          d.z = pack2_bf16(__uint_as_float(o[8 * i + 4]) * inv, __uint_as_float(o[8 * i + 5]) * inv);
-          d.w = pack2_bf16(__uint_as_float(o[8 * i + 6]) * inv, __uint_as_float(o[8 * i + 7]) * inv);
-          if (on) *reinterpret_cast<uint4*>(dst + 32 * c + 8 * i) = d;
+        for (int i = 0; i < 16; ++i) d[i] = pack2_bf16(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {                         // pieces 2, 3 of the lower lanes against 0, 1 of the upper ones
+          const uint32_t got = __shfl_xor_sync(0xffffffffu, hi ? d[i] : d[8 + i], 16);
+          if (hi) d[i] = got; else d[8 + i] = got;
         }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int at = (i >> 2) * 8 + (i & 3);
+          const uint32_t got = __shfl_xor_sync(0xffffffffu, mid ? d[at] : d[at + 4], 8);
+          if (mid) d[at] = got; else d[at + 4] = got;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (dst[i]) *reinterpret_cast<uint4*>(dst[i] + 32 * c) = make_uint4(d[4 * i], d[4 * i + 1], d[4 * i + 2], d[4 * i + 3]);
       }
       tc_fence_before();
     }
@@ -422,6 +435,7 @@ int msa::first_attn_tc(const msa_lm_attn_args& a, int first, int n_rows, int n_c
   const int span = (kFtRows * kFtTiles) >> pack;
   p.n_sh = (long long)(a.seq1 - a.seq0) * (a.heads >> pack);
   p.n_items = p.n_sh * ((a.max_len + span - 1) / span);
+  MSA_REQUIRE(p.n_items < (1ll << 31), "window_attn_tc: too many rows");
   p.out = (__nv_bfloat16*)a.out; p.out_row = a.out_row; p.status = status;
   CUtensorMap mq, mk[3], mv[3];
   MSA_OK_OR_RETURN(make_map_heads(&mq, a.qa, n_rows, a.heads, a.da, a.qa_row, a.qa_head, 1u << pack, (uint32_t)kFtRows >> pack));
