@@ -6,7 +6,7 @@
 // Work item = 256 rows, two tiles of 128 that share every key / value tile on its way through shared memory.  A row is a token and
 // one of 2^pack heads of a key head (as many as the group has factors of two, up to 32): a tile then spans fewer tokens, and fewer
 // keys lie outside a row's window.  One persistent CTA per SM, 320 threads: warps 0-3 the softmax of tile 0, 4-7 that of tile 1 (thread =
-// row = TMEM lane), warp 8 the TMA producer, warp 9 the MMA issuer.  Per 128 keys and row tile:
+// row = TMEM lane), warp 8 the TMA producer, warp 9 the MMA issuer, warp 10 finds the items.  Per 128 keys and row tile:
 //     S = Q K^T    fp32 into the tile's 128 TMEM columns;
 //     softmax      fp32; the reference moves only when the maximum is 2^32 above it (fp32 sums and bf16 weights keep their relative
 //                  precision up to there, and O is rescaled all but never); P as bf16 over the consumed columns;
@@ -24,7 +24,8 @@
 namespace msa {
 
 constexpr int kFtRows = 128, kFtTiles = 2, kFtKeys = 128;
-constexpr int kFtThreads = 32 * (4 * kFtTiles + 2);
+constexpr int kFtThreads = 32 * (4 * kFtTiles + 3);
+constexpr int kFtRing = 4;                                // items known ahead
 constexpr int kFtBlk = kFtRows * 128;                     // one 64-column block of a row, key or value tile: 16 KB
 constexpr int kFtKeyBufs = 3;
 constexpr uint32_t kFtTmem = 512, kFtColO = kFtTiles * kFtKeys;
@@ -101,6 +102,8 @@ first_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
   __shared__ uint64_t s_s_full[kFtTiles], s_p_full[kFtTiles], s_o_full[kFtTiles];
   __shared__ uint32_t s_tmem_base;
   __shared__ int s_abort;
+  __shared__ FtItem s_item[kFtRing];
+  __shared__ uint64_t s_item_full[kFtRing], s_item_empty[kFtRing];
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   unsigned char* tiles = reinterpret_cast<unsigned char*>(((uintptr_t)smem_dyn + 1023) & ~(uintptr_t)1023);
@@ -115,6 +118,7 @@ first_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     for (int q = 0; q < kFtTiles; ++q) {
       mbar_init(&s_s_full[q], 1); mbar_init(&s_p_full[q], 4); mbar_init(&s_o_full[q], 1);
     }
+    for (int i = 0; i < kFtRing; ++i) { mbar_init(&s_item_full[i], 1); mbar_init(&s_item_empty[i], 4 * kFtTiles + 2); }
     s_abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -128,12 +132,30 @@ first_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
   tc_fence_after();
   const uint32_t tmem_base = s_tmem_base;
 
-  // Every role walks the same items.  Keys come one tile ahead of their values: an item starts with its queries and first keys, and turn t
+  // Every role walks the same items, which warp 10 puts into a ring: found by the roles themselves, each item began with 1500 to 3500 cycles
+  // of loads behind the last one's stores.  Keys come one tile ahead of their values: an item starts with its queries and first keys, and turn t
   // brings the values of tile t with the keys of tile t + 1.  n_t counts the turns (stage and phase of the K / V barriers), n_c the tiles
   // that a row tile took part in (phase of its S and P barriers), n_o its items, n_it all items.  Turn n_t waits for the end of turn n_t - 2,
   // in front of which S of an item's first keys may not have been issued: three buffers of keys, taken in turn (b_k), so that
   // those are overwritten two turns after S's own.
-  if (warp == 4 * kFtTiles) {
+  auto item_wait = [&](uint32_t n) { return mbar_wait(&s_item_full[n % kFtRing], (n / kFtRing) & 1u, abort_flag, p.status, 7); };
+  if (warp == 4 * kFtTiles + 2) {
+    if (lane == 0) {
+      uint32_t n = 0;
+      for (long long w = blockIdx.x;; w += gridDim.x) {
+        FtItem it{};                                          // behind the last one: not valid, which ends the walk
+        if (w < p.n_items) {
+          it = ft_item(p, w);
+          if (!it.valid) continue;
+        }
+        if (!mbar_wait(&s_item_empty[n % kFtRing], ((n / kFtRing) & 1u) ^ 1u, abort_flag, p.status, 7)) break;
+        s_item[n % kFtRing] = it;
+        mbar_arrive(&s_item_full[n % kFtRing]);
+        ++n;
+        if (w >= p.n_items) break;
+      }
+    }
+  } else if (warp == 4 * kFtTiles) {
     if (lane == 0) {
       uint32_t n_it = 0, n_t = 0, b_k = 0;
       bool ok = true;
@@ -152,9 +174,10 @@ first_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
           }
         }
       };
-      for (long long w = blockIdx.x; w < p.n_items && ok; w += gridDim.x) {
-        const FtItem it = ft_item(p, w);
-        if (!it.valid) continue;
+      while (ok && (ok = item_wait(n_it))) {
+        const FtItem it = s_item[n_it % kFtRing];
+        mbar_arrive(&s_item_empty[n_it % kFtRing]);
+        if (!it.valid) break;
         if (!(ok = mbar_wait(&s_q_empty, (n_it & 1u) ^ 1u, abort_flag, p.status, 1))) break;
         const int k_col = it.h / p.group * p.k_head, v_col = it.h / p.group * p.v_head;
         mbar_expect_tx(&s_q_full, (kFtTiles + 1) * DB * kFtBlk);
@@ -202,9 +225,10 @@ first_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
                         b_desc + (uint64_t)((c * kFtBlk >> 4) + 2 * k), idesc_s, (c > 0 || k > 0) ? 1u : 0u);
         tc_commit(&s_s_full[q]);
       };
-      for (long long w = blockIdx.x; w < p.n_items && ok; w += gridDim.x) {
-        const FtItem it = ft_item(p, w);
-        if (!it.valid) continue;
+      while (ok && (ok = item_wait(n_it))) {
+        const FtItem it = s_item[n_it % kFtRing];
+        mbar_arrive(&s_item_empty[n_it % kFtRing]);
+        if (!it.valid) break;
         if (!(ok = mbar_wait(&s_q_full, n_it & 1u, abort_flag, p.status, 2))) break;
         tc_fence_after();
 #pragma unroll
@@ -248,15 +272,28 @@ first_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     const uint32_t s_addr = lane_base + (uint32_t)(q * kFtKeys), o_addr = lane_base + kFtColO + (uint32_t)(q * VB * 64);
     uint32_t n_c = 0, n_o = 0;
     bool ok = true;
-    for (long long w = blockIdx.x; w < p.n_items && ok; w += gridDim.x) {
-      const FtItem it = ft_item(p, w);
+    for (uint32_t n_it = 0; ok; ++n_it) {
+      ok = item_wait(n_it);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      const FtItem& ring = s_item[n_it % kFtRing];
+      struct { int len, tok0, h, q_row, old, shift; } it = {ring.len, ring.tok0, ring.h, ring.q_row, ring.old, ring.shift};
+      const int f_q = ring.f[q], a_q = ring.a[q], b_q = ring.b[q];
+      const bool more = ring.valid;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s_item_empty[n_it % kFtRing]);
+      if (!more) break;
       const int t_first = it.tok0 + q * (kFtRows >> p.pack);
-      if (!it.valid || t_first >= it.len) continue;
+      if (t_first >= it.len) continue;
+      const int r_first = it.q_row - it.tok0 + t_first;       // row of the tile's first token in q and out
+      const int low = (1 << p.pack) - 1, r_mine = wq * 32 + lane;
+      float gate = INFINITY;
+      if (p.gate && t_first + (r_mine >> p.pack) < it.len)
+        gate = __bfloat162float(p.gate[(long long)(r_first + (r_mine >> p.pack)) * p.gate_row + it.h + (r_mine & low)]);
       float m_ref = p.sink ? 0.f : -1e30f, l_run = p.sink ? 1.f : 0.f;
       const int row0 = t_first + ((wq * 32) >> p.pack), row1 = t_first + ((wq * 32 + 31) >> p.pack);   // this warp's tokens
       const int mine = it.old + t_first + ((wq * 32 + lane) >> p.pack);                                // context row of the lane's token
       bool joined = false;                                    // O holds something of this item
-      const int f_q = q ? it.f[1] : it.f[0], a_q = q ? it.a[1] : it.a[0], b_q = q ? it.b[1] : it.b[0];
       for (int t = 0; t < b_q; t = t + 1 < f_q || t + 1 >= a_q ? t + 1 : a_q) {
         ok = mbar_wait(&s_s_full[q], n_c & 1u, abort_flag, p.status, 5);
         ok = __all_sync(0xffffffffu, ok);
@@ -345,11 +382,7 @@ first_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
-      const int r_first = it.q_row - it.tok0 + t_first;       // row of the tile's first token in q and out
-      const int low = (1 << p.pack) - 1, r_mine = wq * 32 + lane;
-      float inv = 1.f / l_run;
-      if (p.gate && t_first + (r_mine >> p.pack) < it.len)
-        inv *= sigmoid_f(__bfloat162float(p.gate[(long long)(r_first + (r_mine >> p.pack)) * p.gate_row + it.h + (r_mine & low)]));
+      const float inv = sigmoid_f(gate) / l_run;              // sigmoid(inf) = 1
       // Eight rows of 64 bytes a store: lanes trade the 16-byte pieces of their rows, the piece's two bits for the lane's upper two.
       const int hi = lane >> 4, mid = (lane >> 3) & 1, piece = lane >> 3;
       __nv_bfloat16* dst[4];
