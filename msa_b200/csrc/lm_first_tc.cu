@@ -287,9 +287,10 @@ first_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       if (t_first >= it.len) continue;
       const int r_first = it.q_row - it.tok0 + t_first;       // row of the tile's first token in q and out
       const int low = (1 << p.pack) - 1, r_mine = wq * 32 + lane;
-      float gate = INFINITY;
-      if (p.gate && t_first + (r_mine >> p.pack) < it.len)
-        gate = __bfloat162float(p.gate[(long long)(r_first + (r_mine >> p.pack)) * p.gate_row + it.h + (r_mine & low)]);
+      // The gate is on its way during the tiles; a sigmoid of infinity is 1.
+      const bool gated = p.gate && t_first + (r_mine >> p.pack) < it.len;
+      unsigned short gate = 0x7f80;
+      if (gated) gate = reinterpret_cast<const unsigned short*>(p.gate)[(long long)(r_first + (r_mine >> p.pack)) * p.gate_row + it.h + (r_mine & low)];
       float m_ref = p.sink ? 0.f : -1e30f, l_run = p.sink ? 1.f : 0.f;
       const int row0 = t_first + ((wq * 32) >> p.pack), row1 = t_first + ((wq * 32 + 31) >> p.pack);   // this warp's tokens
       const int mine = it.old + t_first + ((wq * 32 + lane) >> p.pack);                                // context row of the lane's token
@@ -382,7 +383,7 @@ first_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
-      const float inv = sigmoid_f(gate) / l_run;              // sigmoid(inf) = 1
+      const float inv = sigmoid_f(__uint_as_float((uint32_t)gate << 16)) / l_run;
       // Eight rows of 64 bytes a store: lanes trade the 16-byte pieces of their rows, the piece's two bits for the lane's upper two.
       const int hi = lane >> 4, mid = (lane >> 3) & 1, piece = lane >> 3;
       __nv_bfloat16* dst[4];
@@ -391,7 +392,7 @@ first_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         const int r = wq * 32 + 8 * i + (lane & 7), tok = r >> p.pack;
         dst[i] = t_first + tok < it.len ? p.out + (long long)(r_first + tok) * p.out_row + (it.h + (r & low)) * VB * 64 + 8 * piece : nullptr;
       }
-#pragma unroll
+#pragma unroll 1                                              // run once an item: unrolled, it waits for its instructions
       for (int c = 0; c < VB * 2; ++c) {
         uint32_t o[32], d[16];                                // d: [piece][word]
         tmem_ld32(o_addr + 32 * c, o);
