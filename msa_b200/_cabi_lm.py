@@ -168,7 +168,10 @@ def lib() -> C.CDLL:
 
 def on_device(device: torch.device):
     """Makes ``device`` the current one for a launch, if it is not."""
-    return contextlib.nullcontext() if device.index in (None, torch.cuda.current_device()) else torch.cuda.device(device)
+    return _HERE_ALREADY if device.index in (None, torch.cuda.current_device()) else torch.cuda.device(device)
+
+
+_HERE_ALREADY = contextlib.nullcontext()
 
 
 launches = 0    # calls into the library since import (each is one kernel launch)

@@ -187,16 +187,16 @@ def beam_topk(logits: torch.Tensor, scores: torch.Tensor, k: int, stop: Optional
         raise A.MsaError("beam_topk: contiguous scores on the logits' device expected")
     if stop is not None and (stop.device != dev or stop.dtype != torch.int32 or stop.dim() != 1 or not stop.is_contiguous()):
         raise A.MsaError("beam_topk: stop tokens must be a contiguous int32 vector on the logits' device")
-    new = lambda n, dt: torch.empty((batch, n), dtype=dt, device=dev)
-    out = [new(k, torch.float32), new(k, torch.int32), new(k, torch.int32)]
-    if stop is not None:
-        out += [new(beams, torch.float32), new(beams, torch.int32), new(beams, torch.int32)]
+    def new(n):                                                  # three tables from one allocation
+        score, beam, token = torch.empty((3, batch, n), dtype=torch.int32, device=dev).unbind(0)
+        return score.view(torch.float32), beam, token
+    out = new(k) if stop is None else new(k) + new(beams)
     if batch:
         with A.on_device(dev):
             work = torch.empty(A.lib().msa_lm_beam_topk_workspace(batch, beams, vocab, k), dtype=torch.uint8, device=dev)
             A.call("msa_lm_beam_topk", A.ptr(logits), logits.stride(0), A.dtype_code(logits.dtype), A.ptr(scores), batch, beams, vocab, k, A.ptr(stop),
-                   0 if stop is None else stop.shape[0], A.ptr(work), *(A.ptr(t) for t in out), *([0] * (6 - len(out))), A.stream_ptr(dev))
-    return tuple(out)
+                   0 if stop is None else stop.shape[0], A.ptr(work), *(t.data_ptr() for t in out), *((0,) * (6 - len(out))), A.stream_ptr(dev))
+    return out
 
 
 def token_shift(h, mu, step, shift):
@@ -240,19 +240,29 @@ def attn_args(qa, qb, ka, kb, v, out, *, scale, window, start, cu, seq0, seq1, m
               sink=False, gate=None) -> A.AttnArgs:
     """``qa`` / ``qb`` / ``out`` are ``[tokens, heads, d]`` views of the query rows, ``ka`` / ``kb`` / ``v`` ``[rows, kv heads, d]``
     views of the key rows; ``gate`` ``[tokens, heads]`` logits."""
-    head = lambda t: 0 if t is None or t.shape[1] == 1 else t.stride(1)
-    row = lambda t: 0 if t is None else t.stride(0)
-    for t in (qa, qb, ka, kb, v, out):
-        if t is not None and t.stride(2) != 1:
-            raise A.MsaError("window attention: contiguous last axis expected")
+    # positional and from whole strides: as keywords, number by number, the same took 10 us of a small portion's 24, this 5
+    q_row, q_head, q1 = qa.stride()
+    k_row, k_head, k1 = ka.stride()
+    v_row, v_head, v1 = v.stride()
+    o_row, o_head, o1 = out.stride()
+    _, heads, da = qa.shape
+    _, k_heads, _ = ka.shape
+    _, v_heads, dv = v.shape
+    qb_ptr = qb_row = qb_head = kb_ptr = kb_row = kb_head = db = 0
+    if qb is not None:
+        qb_row, qb_head, b1 = qb.stride()
+        qb_ptr, db, q1 = qb.data_ptr(), qb.shape[2], q1 if b1 == 1 else b1
+    if kb is not None:
+        kb_row, kb_head, b1 = kb.stride()
+        kb_ptr, kb_head, k1 = kb.data_ptr(), 0 if kb.shape[1] == 1 else kb_head, k1 if b1 == 1 else b1
+    if not q1 == k1 == v1 == o1 == 1:
+        raise A.MsaError("window attention: contiguous last axis expected")
+    ptr = A.ptr
     return A.AttnArgs(
-        qa=A.ptr(qa), qa_row=row(qa), qa_head=qa.stride(1), qb=A.ptr(qb), qb_row=row(qb), qb_head=qb.stride(1) if qb is not None else 0,
-        ka=A.ptr(ka), ka_row=row(ka), ka_head=head(ka), kb=A.ptr(kb), kb_row=row(kb), kb_head=head(kb),
-        v=A.ptr(v), v_row=row(v), v_head=head(v), out=A.ptr(out), out_row=row(out), out_head=out.stride(1),
-        gate=A.ptr(gate), gate_row=row(gate), slot=A.ptr(slot), start=A.ptr(start), cu=A.ptr(cu), ctx_off=A.ptr(ctx_off),
-        ring_rows=ring_rows, group=qa.shape[1] // max(ka.shape[1], v.shape[1]), sink=1 if sink else 0, seq0=seq0, seq1=seq1,
-        max_len=max_len, heads=qa.shape[1], da=qa.shape[2], db=qb.shape[2] if qb is not None else 0, dv=v.shape[2], window=window,
-        qa_dtype=A.dtype_code(qa.dtype), out_dtype=A.dtype_code(out.dtype), dtype=A.dtype_code(ka.dtype), scale=float(scale))
+        qa.data_ptr(), q_row, q_head, qb_ptr, qb_row, qb_head, ka.data_ptr(), k_row, 0 if k_heads == 1 else k_head, kb_ptr, kb_row, kb_head,
+        v.data_ptr(), v_row, 0 if v_heads == 1 else v_head, out.data_ptr(), o_row, o_head, ptr(gate), 0 if gate is None else gate.stride(0),
+        ptr(slot), ptr(start), ptr(cu), ptr(ctx_off), ring_rows, heads // max(k_heads, v_heads), 1 if sink else 0, seq0, seq1, max_len,
+        heads, da, db, dv, window, A.dtype_code(qa.dtype), A.dtype_code(out.dtype), A.dtype_code(ka.dtype), scale)
 
 
 def window_attn(qa, qb, ka, kb, v, out, *, first=0, **kw):
@@ -331,13 +341,14 @@ def group_decode(q, ring, kv_heads, step, out, *, window, scale, sink, gate, fir
     n, heads, dim = q.shape
     vdim = out.shape[2]
     splits = group_decode_splits(n, heads, kv_heads, ring.shape[1])
-    part_o = part_ml = None
-    if splits > 1:
-        f = dict(dtype=torch.float32, device=q.device)
-        part_o, part_ml = torch.empty((n, heads, splits, vdim), **f), torch.empty((n, heads, splits, 2), **f)
+    part_o = part_ml = 0
+    if splits > 1:                                               # one allocation for both
+        work = torch.empty(n * heads * splits * (vdim + 2), dtype=torch.float32, device=q.device)
+        part_o = work.data_ptr()
+        part_ml = part_o + n * heads * splits * vdim * 4
     A.call("msa_lm_group_decode_first", A.ptr(q), q.stride(0), A.ptr(ring), ring.shape[1], A.ptr(step.slot), A.ptr(step.start), n, heads, kv_heads, dim,
            vdim, window, first, splits, float(scale), 1 if sink else 0, A.ptr(gate), gate.stride(0) if gate is not None else 0, A.ptr(out),
-           out.stride(0), A.ptr(part_o), A.ptr(part_ml), A.stream_ptr(q.device))
+           out.stride(0), part_o, part_ml, A.stream_ptr(q.device))
 
 
 # ---------------------------------------------------------------------------------------------- decaying outer products
