@@ -142,7 +142,8 @@ int msa_lm_group_prep(const msa_lm_group_args* args, void* stream);
  * The functions without `first` are those of first = 0.  With it, position i sees j <= i with i - j < window or j < first.  A ring
  * (of first + window rows at least) keeps position p in row p while p < first, and in row first + (p - first) % (ring_rows - first)
  * from there on.  The context of a portion begins with the min(start, first + window - 1) earlier positions that its first
- * token sees: the first tokens, then the window; its own rows follow. */
+ * token sees: the first tokens, then the window; its own rows follow.  group_decode_first with up to 8 splits and null part_o and
+ * part_ml joins the splits in the same launch. */
 int msa_lm_group_prep_first(const msa_lm_group_args* args, int32_t first, void* stream);
 int msa_lm_ring_store_first(const void* ctx, int32_t row_width, const int32_t* slot, const int32_t* start, const int32_t* cu,
                             const int32_t* ctx_off, int32_t n_seq, int32_t n_decode, int32_t max_len, int32_t window, int32_t first,

@@ -335,6 +335,16 @@ def group_decode_splits(n: int, heads: int, kv_heads: int, ring_rows: int, n_sm:
     return max(1, min(2 * n_sm // max(n * tiles, 1), (ring_rows + 63) // 64, 64))
 
 
+GROUP_CLUSTER = 8            # splits of a cluster, at most
+
+
+def splits_join(splits: int, ring_rows: int) -> bool:
+    """Whether a cluster of up to 8 splits, which joins its results in the same launch, beats more of them with a kernel that merges.  16 heads
+    over 4 of 128, one sequence: 12.3 us against 14.3 over 1028 rows, 16.4 against 20.5 over 4100, 22.5 both over 8196 and 32.8 against 24.6 over
+    16,388; 16 sequences, 4 splits in either form: 18.4 against 20.5 over 1028 and 114.7 against 116.7 over 16,388."""
+    return splits <= GROUP_CLUSTER or ring_rows <= 4608
+
+
 def group_decode(q, ring, kv_heads, step, out, *, window, scale, sink, gate, first=0):
     """``q`` [n, heads, dim], ``out`` [n, heads, vdim] views, ``ring`` [slots, rows, kv_heads * (dim + vdim)]; ``first``: tokens that
     stay visible in front of the window."""
@@ -342,7 +352,9 @@ def group_decode(q, ring, kv_heads, step, out, *, window, scale, sink, gate, fir
     vdim = out.shape[2]
     splits = group_decode_splits(n, heads, kv_heads, ring.shape[1])
     part_o = part_ml = 0
-    if splits > 1:                                               # one allocation for both
+    if first and splits_join(splits, ring.shape[1]):
+        splits = min(splits, GROUP_CLUSTER)
+    elif splits > 1:                                             # one allocation for both
         work = torch.empty(n * heads * splits * (vdim + 2), dtype=torch.float32, device=q.device)
         part_o = work.data_ptr()
         part_ml = part_o + n * heads * splits * vdim * 4
