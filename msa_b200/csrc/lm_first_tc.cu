@@ -5,8 +5,8 @@
 //
 // Work item = 256 rows, two tiles of 128 that share every key / value tile on its way through shared memory.  A row is a token and
 // one of 2^pack heads of a key head (as many as the group has factors of two, up to 32): a tile then spans fewer tokens, and fewer
-// keys lie outside a row's window.  One persistent CTA per SM, 320 threads: warps 0-3 the softmax of tile 0, 4-7 that of tile 1 (thread =
-// row = TMEM lane), warp 8 the TMA producer, warp 9 the MMA issuer, warp 10 finds the items.  Per 128 keys and row tile:
+// keys lie outside a row's window.  One persistent CTA per SM, 384 threads: warps 0-3 the softmax of tile 0, 4-7 that of tile 1 (thread =
+// row = TMEM lane), warp 8 the TMA producer, warp 9 the MMA issuer, warp 10 finds the items, warp 11 clears values that are not the sequence's own.  Per 128 keys and row tile:
 //     S = Q K^T    fp32 into the tile's 128 TMEM columns;
 //     softmax      fp32; the reference moves only when the maximum is 2^32 above it (fp32 sums and bf16 weights keep their relative
 //                  precision up to there, and O is rescaled all but never); P as bf16 over the consumed columns;
@@ -24,7 +24,7 @@
 namespace msa {
 
 constexpr int kFtRows = 128, kFtTiles = 2, kFtKeys = 128;
-constexpr int kFtThreads = 32 * (4 * kFtTiles + 3);
+constexpr int kFtThreads = 32 * (4 * kFtTiles + 4);
 constexpr int kFtRing = 4;                                // items known ahead
 constexpr int kFtBlk = kFtRows * 128;                     // one 64-column block of a row, key or value tile: 16 KB
 constexpr int kFtKeyBufs = 3;
@@ -49,8 +49,10 @@ struct FirstAttnParams {
 // Items are numbered from every portion's last block to its first: the late ones see the most keys, and the fixed-stride walk of the
 // persistent CTAs then ends on short ones.  Row tile q takes part in the key tiles below f[q] and in a[q] .. b[q]-1.
 struct FtItem {
-  int len, tok0, h, q_row, ctx, old, shift, n_kt, f[kFtTiles], a[kFtTiles], b[kFtTiles];
+  int len, tok0, h, q_row, ctx, old, shift, own, n_kt, f[kFtTiles], a[kFtTiles], b[kFtTiles];   // own: slots in front of the context's end
+  uint32_t turn;                                             // turns of the items before it
   bool valid;
+  __device__ __forceinline__ bool foreign() const { return own < n_kt * kFtKeys; }       // rows in the last key tile
   __device__ __forceinline__ bool has(int q, int t) const { return t < f[q] || (t >= a[q] && t < b[q]); }
 };
 __device__ __forceinline__ FtItem ft_item(const FirstAttnParams& p, long long w) {
@@ -68,6 +70,7 @@ __device__ __forceinline__ FtItem ft_item(const FirstAttnParams& p, long long w)
   it.q_row = c0 - p.q_row0 + it.tok0;
   it.ctx = p.ctx_off[ps];
   it.shift = max(p.pad, it.old + it.tok0 - p.window + 1) - p.pad;      // context row = slot + shift behind the first rows
+  it.own = it.old + it.len - it.shift;
   it.n_kt = 0;
 #pragma unroll
   for (int q = 0; q < kFtTiles; ++q) {
@@ -91,6 +94,16 @@ __device__ __forceinline__ uint32_t slot_bits(int lo, int hi, int s0) {
   return below_h & ~below_l;
 }
 
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
+}
+// A store that leaves no line in the L1, which shared memory holds nearly all of: 5 us of 262 for portions of 4 x 2048 tokens.
+__device__ __forceinline__ void store_once(void* p, uint4 v) {
+  asm volatile("st.global.L1::no_allocate.v4.b32 [%0], {%1, %2, %3, %4};" ::"l"(p), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
 template <int DB, int VB>
 __global__ void __launch_bounds__(kFtThreads, 1)
 first_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_k0,
@@ -98,7 +111,7 @@ first_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
                      const __grid_constant__ CUtensorMap tmap_v1, const FirstAttnParams p) {
   static_assert(kFtColO + kFtTiles * VB * 64 <= kFtTmem, "TMEM columns");
   extern __shared__ unsigned char smem_dyn[];
-  __shared__ uint64_t s_q_full, s_q_empty, s_kv_full[2], s_kv_empty[2], s_drain;
+  __shared__ uint64_t s_q_full, s_q_empty, s_kv_full[2], s_kv_empty[2], s_dirty, s_clean, s_drain;
   __shared__ uint64_t s_s_full[kFtTiles], s_p_full[kFtTiles], s_o_full[kFtTiles];
   __shared__ uint32_t s_tmem_base;
   __shared__ int s_abort;
@@ -113,12 +126,12 @@ first_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
   volatile int* abort_flag = &s_abort;
 
   if (threadIdx.x == 0) {
-    mbar_init(&s_q_full, 1); mbar_init(&s_q_empty, 1); mbar_init(&s_drain, 1);
+    mbar_init(&s_q_full, 1); mbar_init(&s_q_empty, 1); mbar_init(&s_dirty, 1); mbar_init(&s_clean, 1); mbar_init(&s_drain, 1);
     for (int i = 0; i < 2; ++i) { mbar_init(&s_kv_full[i], 1); mbar_init(&s_kv_empty[i], 1); }
     for (int q = 0; q < kFtTiles; ++q) {
       mbar_init(&s_s_full[q], 1); mbar_init(&s_p_full[q], 4); mbar_init(&s_o_full[q], 1);
     }
-    for (int i = 0; i < kFtRing; ++i) { mbar_init(&s_item_full[i], 1); mbar_init(&s_item_empty[i], 4 * kFtTiles + 2); }
+    for (int i = 0; i < kFtRing; ++i) { mbar_init(&s_item_full[i], 1); mbar_init(&s_item_empty[i], 4 * kFtTiles + 3); }
     s_abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -141,7 +154,7 @@ first_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
   auto item_wait = [&](uint32_t n) { return mbar_wait(&s_item_full[n % kFtRing], (n / kFtRing) & 1u, abort_flag, p.status, 7); };
   if (warp == 4 * kFtTiles + 2) {
     if (lane == 0) {
-      uint32_t n = 0;
+      uint32_t n = 0, turn = 0;
       for (long long w = blockIdx.x;; w += gridDim.x) {
         FtItem it{};                                          // behind the last one: not valid, which ends the walk
         if (w < p.n_items) {
@@ -149,11 +162,38 @@ first_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
           if (!it.valid) continue;
         }
         if (!mbar_wait(&s_item_empty[n % kFtRing], ((n / kFtRing) & 1u) ^ 1u, abort_flag, p.status, 7)) break;
+        it.turn = turn;
+        turn += (uint32_t)it.n_kt;
         s_item[n % kFtRing] = it;
         mbar_arrive(&s_item_full[n % kFtRing]);
         ++n;
         if (w >= p.n_items) break;
       }
+    }
+  } else if (warp == 4 * kFtTiles + 3) {
+    // Rows behind the portion's context belong to another sequence, or to nobody.  Their weights are 0, which would still take an infinity or
+    // a NaN from their values into the product: they are cleared before it.  (By the softmax warps, this cost all tiles 15 us of 265.)
+    bool ok = true;
+    uint32_t n_cl = 0;
+    for (uint32_t n_it = 0; ok; ++n_it) {
+      ok = __all_sync(0xffffffffu, item_wait(n_it));
+      if (!ok) break;
+      const FtItem& it = s_item[n_it % kFtRing];
+      const bool more = it.valid, foreign = it.foreign();
+      const int own = it.own - (it.n_kt - 1) * kFtKeys;
+      const uint32_t n = it.turn + (uint32_t)it.n_kt - 1u;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s_item_empty[n_it % kFtRing]);
+      if (!more) break;
+      if (!foreign) continue;
+      ok = __all_sync(0xffffffffu, mbar_wait(&s_dirty, n_cl++ & 1u, abort_flag, p.status, 8));      // the tile has come
+      if (!ok) break;
+      for (int i = own * 8 + lane; i < kFtKeys * 8; i += 32)
+#pragma unroll
+        for (int c = 0; c < VB; ++c) *reinterpret_cast<uint4*>(v_smem + ((n & 1u) * VB + c) * kFtBlk + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s_clean);
     }
   } else if (warp == 4 * kFtTiles) {
     if (lane == 0) {
@@ -207,65 +247,76 @@ first_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       }
     }
   } else if (warp == 4 * kFtTiles + 1) {
-    if (lane == 0) {
-      const uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kFtKeys >> 3) << 17) | ((uint32_t)(kFtRows >> 4) << 24);
-      const uint32_t idesc_pv = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(VB * 64 >> 3) << 17) |
-                                ((uint32_t)(kFtRows >> 4) << 24);
-      const uint64_t q_desc = make_smem_desc(smem_u32(q_smem)), k_desc = make_smem_desc(smem_u32(k_smem)),
-                     v_desc = make_smem_desc_mn(smem_u32(v_smem), kFtBlk);
-      uint32_t n_it = 0, n_t = 0, b_k = 0, n_p[kFtTiles] = {};   // n_p: PV tiles issued so far
-      bool ok = true;
-      auto issue_s = [&](uint32_t g, int q) {                // S of the keys in buffer g for row tile q
-        const uint64_t b_desc = k_desc + (uint64_t)(g * (DB * kFtBlk >> 4));
+    // The whole warp walks along, and one thread (always the same) issues: with the others left behind at a branch around all of this, each
+    // product's descriptors cost more than the product (261 us where this takes 256).
+    const uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kFtKeys >> 3) << 17) | ((uint32_t)(kFtRows >> 4) << 24);
+    const uint32_t idesc_pv = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(VB * 64 >> 3) << 17) |
+                              ((uint32_t)(kFtRows >> 4) << 24);
+    const uint64_t q_desc = make_smem_desc(smem_u32(q_smem)), k_desc = make_smem_desc(smem_u32(k_smem)),
+                   v_desc = make_smem_desc_mn(smem_u32(v_smem), kFtBlk);
+    uint32_t n_it = 0, n_t = 0, n_cl = 0, b_k = 0, n_p[kFtTiles] = {};   // n_cl: tiles that were cleared, n_p: PV tiles issued so far
+    bool ok = true;
+    auto all_wait = [&](uint64_t* bar, uint32_t ph, int code) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, ph, abort_flag, p.status, code)); };
+    auto issue_s = [&](uint32_t g, int q) {                // S of the keys in buffer g for row tile q
+      if (!elect_one()) return;
+      const uint64_t b_desc = k_desc + (uint64_t)(g * (DB * kFtBlk >> 4));
 #pragma unroll
-        for (int c = 0; c < DB; ++c)
+      for (int c = 0; c < DB; ++c)
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            tc_mma_bf16(tmem_base + (uint32_t)(q * kFtKeys), q_desc + (uint64_t)(((q * DB + c) * kFtBlk >> 4) + 2 * k),
-                        b_desc + (uint64_t)((c * kFtBlk >> 4) + 2 * k), idesc_s, (c > 0 || k > 0) ? 1u : 0u);
-        tc_commit(&s_s_full[q]);
-      };
-      while (ok && (ok = item_wait(n_it))) {
-        const FtItem it = s_item[n_it % kFtRing];
-        mbar_arrive(&s_item_empty[n_it % kFtRing]);
-        if (!it.valid) break;
-        if (!(ok = mbar_wait(&s_q_full, n_it & 1u, abort_flag, p.status, 2))) break;
-        tc_fence_after();
+        for (int k = 0; k < 4; ++k)
+          tc_mma_bf16(tmem_base + (uint32_t)(q * kFtKeys), q_desc + (uint64_t)(((q * DB + c) * kFtBlk >> 4) + 2 * k),
+                      b_desc + (uint64_t)((c * kFtBlk >> 4) + 2 * k), idesc_s, (c > 0 || k > 0) ? 1u : 0u);
+      tc_commit(&s_s_full[q]);
+    };
+    while (ok && (ok = __all_sync(0xffffffffu, item_wait(n_it)))) {
+      const FtItem it = s_item[n_it % kFtRing];
+      __syncwarp();
+      if (elect_one()) mbar_arrive(&s_item_empty[n_it % kFtRing]);
+      if (!it.valid) break;
+      if (!(ok = all_wait(&s_q_full, n_it & 1u, 2))) break;
+      tc_fence_after();
 #pragma unroll
-        for (int q = 0; q < kFtTiles; ++q)
-          if (it.has(q, 0)) issue_s(b_k, q);                  // behind the last item's products that read these columns
-        b_k = b_k + 1 == kFtKeyBufs ? 0u : b_k + 1;
-        if (it.n_kt == 1) tc_commit(&s_q_empty);
-        for (int t = 0; t < it.n_kt; ++t, ++n_t) {
-          const uint32_t st = n_t & 1u;
-          const bool more = t + 1 < it.n_kt;
-          if (!(ok = mbar_wait(&s_kv_full[st], (n_t >> 1) & 1u, abort_flag, p.status, 3))) break;
-          const uint64_t b_desc = v_desc + (uint64_t)(st * (VB * kFtBlk >> 4));
+      for (int q = 0; q < kFtTiles; ++q)
+        if (it.has(q, 0)) issue_s(b_k, q);                  // behind the last item's products that read these columns
+      b_k = b_k + 1 == kFtKeyBufs ? 0u : b_k + 1;
+      if (it.n_kt == 1 && elect_one()) tc_commit(&s_q_empty);
+      for (int t = 0; t < it.n_kt; ++t, ++n_t) {
+        const uint32_t st = n_t & 1u;
+        const bool more = t + 1 < it.n_kt;
+        if (!(ok = all_wait(&s_kv_full[st], (n_t >> 1) & 1u, 3))) break;
+        if (!more && it.foreign()) {
+          if (elect_one()) mbar_arrive(&s_dirty);
+          if (!(ok = all_wait(&s_clean, n_cl++ & 1u, 8))) break;
+        }
+        const uint64_t b_desc = v_desc + (uint64_t)(st * (VB * kFtBlk >> 4));
 #pragma unroll
-          for (int q = 0; q < kFtTiles; ++q) {
-            if (it.has(q, t)) {
-              if (!(ok = mbar_wait(&s_p_full[q], n_p[q] & 1u, abort_flag, p.status, 4))) break;
-              tc_fence_after();
+        for (int q = 0; q < kFtTiles; ++q) {
+          if (it.has(q, t)) {
+            if (!(ok = all_wait(&s_p_full[q], n_p[q] & 1u, 4))) break;
+            tc_fence_after();
+            if (elect_one()) {
 #pragma unroll
               for (int j = 0; j < kFtKeys / 16; ++j)
                 tc_mma_bf16_ts(tmem_base + kFtColO + (uint32_t)(q * VB * 64), tmem_base + (uint32_t)(q * kFtKeys + 8 * j), b_desc + (uint64_t)(j * (2048 >> 4)),
                                idesc_pv, t > 0 || j > 0 ? 1u : 0u);
               if (t + 1 == it.b[q]) tc_commit(&s_o_full[q]);
-              ++n_p[q];
             }
-            if (more && it.has(q, t + 1)) issue_s(b_k, q);    // in order behind the PV that read these columns
+            ++n_p[q];
           }
-          if (!ok) break;
-          if (more) b_k = b_k + 1 == kFtKeyBufs ? 0u : b_k + 1;
+          if (more && it.has(q, t + 1)) issue_s(b_k, q);    // in order behind the PV that read these columns
+        }
+        if (!ok) break;
+        if (more) b_k = b_k + 1 == kFtKeyBufs ? 0u : b_k + 1;
+        if (elect_one()) {
           tc_commit(&s_kv_empty[st]);
           if (t + 2 == it.n_kt) tc_commit(&s_q_empty);
         }
-        ++n_it;
       }
-      tc_commit(&s_drain);
-      const unsigned long long w0 = global_ns();
-      while (!mbar_try_wait(&s_drain, 0) && global_ns() - w0 < kWaitLimitNs) {}
+      ++n_it;
     }
+    if (elect_one()) tc_commit(&s_drain);
+    const unsigned long long w0 = global_ns();
+    while (!mbar_try_wait(&s_drain, 0) && global_ns() - w0 < kWaitLimitNs) {}
   } else {
     const int q = warp / 4, wq = warp % 4;
     const uint32_t lane_base = tmem_base + ((uint32_t)(wq * 32) << 16);
@@ -276,15 +327,15 @@ first_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       ok = item_wait(n_it);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
-      const FtItem& ring = s_item[n_it % kFtRing];
-      struct { int len, tok0, h, q_row, old, shift; } it = {ring.len, ring.tok0, ring.h, ring.q_row, ring.old, ring.shift};
-      const int f_q = ring.f[q], a_q = ring.a[q], b_q = ring.b[q];
-      const bool more = ring.valid;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&s_item_empty[n_it % kFtRing]);
-      if (!more) break;
+      const FtItem& it = s_item[n_it % kFtRing];              // kept until the item's end: registers are short
+      if (!it.valid) break;
+      const int f_q = it.f[q], a_q = it.a[q], b_q = it.b[q];
+      auto release = [&] {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_item_empty[n_it % kFtRing]);
+      };
       const int t_first = it.tok0 + q * (kFtRows >> p.pack);
-      if (t_first >= it.len) continue;
+      if (t_first >= it.len) { release(); continue; }
       const int r_first = it.q_row - it.tok0 + t_first;       // row of the tile's first token in q and out
       const int low = (1 << p.pack) - 1, r_mine = wq * 32 + lane;
       // The gate is on its way during the tiles; a sigmoid of infinity is 1.
@@ -412,8 +463,9 @@ first_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (dst[i]) *reinterpret_cast<uint4*>(dst[i] + 32 * c) = make_uint4(d[4 * i], d[4 * i + 1], d[4 * i + 2], d[4 * i + 3]);
+          if (dst[i]) store_once(dst[i] + 32 * c, make_uint4(d[4 * i], d[4 * i + 1], d[4 * i + 2], d[4 * i + 3]));
       }
+      release();
       tc_fence_before();
     }
   }

@@ -221,6 +221,63 @@ def test_tokens_over_the_rings(window, first, dim, vdim, kv, group):
             assert bool((wide[n] == 7.0).all())
 
 
+@pytest.mark.parametrize("n,window,splits", [(2, 5000, 64), (150, 120, 1), (40, 400, 3), (3, 3000, 8)])
+def test_tokens_in_every_number_of_splits(n, window, splits):
+    """One block a sequence, a cluster of blocks, and more blocks than a cluster holds."""
+    from types import SimpleNamespace
+    from msa_b200 import lm_ops as K
+    first, kv, group, dim = 4, 2, 4, 64
+    rows_ = window + first
+    got = K.group_decode_splits(n, kv * group, kv, rows_)
+    assert (min(got, K.GROUP_CLUSTER) if K.splits_join(got, rows_) else got) == splits
+    g = torch.Generator(device=DEV).manual_seed(n)
+    ring = randn(g, n, rows_, kv * 2 * dim)
+    pos = torch.randint(0, 3 * window, (n,), generator=g, device=DEV).to(torch.int32)
+    pos[0], pos[-1] = 0, 50 * window                                 # one row for all the splits; all of them full
+    step = SimpleNamespace(slot=torch.randperm(n, generator=g, device=DEV).to(torch.int32), start=pos)
+    q, gate, out = randn(g, n, kv * group, dim, scale=1.5), randn(g, n, kv * group), torch.empty((n, kv * group, dim), dtype=BF16, device=DEV)
+    for sink in (True, False):
+        K.group_decode(q, ring, kv, step, out, window=window, first=first, scale=dim ** -0.5, sink=sink, gate=gate)
+        for i, p in enumerate(pos.tolist()):
+            j = torch.arange(p + 1, device=DEV)
+            j = j[(j < first) | (p - j < window)]
+            r = ring[int(step.slot[i]), torch.where(j < first, j, first + (j - first) % window)]
+            want, size = attend(q[i:i + 1], r[:, :kv * dim].unflatten(1, (kv, dim)), r[:, kv * dim:].unflatten(1, (kv, dim)),
+                                torch.ones((1, len(j)), dtype=torch.bool, device=DEV), dim ** -0.5, sink, gate[i:i + 1])
+            within(out[i:i + 1], want, size)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("window,first,portions", [(100, 4, "5@0,2@3,130@0,64@300,128@0"), (130, 200, "3@0,70@0,260@500,2@7"), (300, 1, "128@0,384@0,129@129")])
+def test_portions_take_nothing_from_each_other(window, first, portions, bad):
+    """What lies in the others' contexts, or in unused rows behind the last one, does not reach a portion's rows: not a bit of them."""
+    from msa_b200.cache import PackedStep, RingSpec, SequenceStateCache
+    from msa_b200.hybrid import portion_attention
+    parts = [tuple(map(int, p.split("@"))) for p in portions.split(",")]
+    kv, group, dim, vdim = 2, 4, 64, 128
+    cache = SequenceStateCache([RingSpec(8, window, first=first)], len(parts), max(n + s for n, s in parts) + window + first, DEV, BF16)
+    for i, (_, s) in enumerate(parts):
+        cache.acquire(i)
+        cache.advance(i, s)
+    step = PackedStep([(i, [0] * n, []) for i, (n, _) in enumerate(parts)], cache, ((window, first),))
+    view, status = step.views[window, first], torch.zeros(4, dtype=torch.int32, device=DEV)
+    g = torch.Generator(device=DEV).manual_seed(window)
+    q, rows_ = randn(g, step.n_tok, kv * group, dim, scale=1.5), randn(g, view.n_ctx + 300, kv * (dim + vdim))
+
+    def run(all_rows):
+        ctx, out = all_rows[:view.n_ctx], torch.empty((step.n_tok, kv * group, vdim), dtype=BF16, device=DEV)
+        k, v = ctx[:, :kv * dim].unflatten(1, (kv, dim)), ctx[:, kv * dim:].unflatten(1, (kv, vdim))
+        portion_attention((q, None, k, None, v, out), True, status, step, view, dim ** -0.5)
+        return out
+    want, cu, off = run(rows_), step.cu.tolist(), view.ctx_off.tolist()
+    assert bool(want.isfinite().all())
+    for i in range(len(parts)):
+        mixed = torch.full_like(rows_, bad)
+        mixed[off[i]:off[i + 1]] = rows_[off[i]:off[i + 1]]
+        assert torch.equal(run(mixed)[cu[i]:cu[i + 1]], want[cu[i]:cu[i + 1]]), parts[i]
+    assert status.tolist() == [0, 0, 0, 0]
+
+
 # ------------------------------------------------------------------------------------------ a model with such layers
 CONFIG = U.parallel(256, 320, [
     U.layer("attention", attention(8, 2, 64, 128, 40, 4, 32, 4), U.dense(256)),
