@@ -174,7 +174,32 @@ def on_device(device: torch.device):
 _HERE_ALREADY = contextlib.nullcontext()
 
 
+_native = None
+
+
+def native():
+    """The native host side of the calls that are shorter than Python's part in them (``csrc/host_layer.cpp``).  Its functions answer None or
+    False for operands that they do not take, without having launched anything."""
+    global _native
+    if _native is None:
+        lib()
+        from . import _cabi
+        n = _cabi.native()
+        n.bind_lm(LIB_PATH)
+        _native = n
+    return _native
+
+
 launches = 0    # calls into the library since import (each is one kernel launch)
+
+
+def count(done) -> bool:
+    """Whether a native function has made its call, which then counts."""
+    global launches
+    if done is None or done is False:
+        return False
+    launches += 1
+    return True
 
 
 def call(name: str, *args) -> None:

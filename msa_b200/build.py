@@ -31,7 +31,7 @@ LIBRARIES = {
 
 
 NATIVE_SOURCE = "host_layer.cpp"
-LIBRARIES["native"] = (None, [NATIVE_SOURCE], [], ["msa_b200.h"])      # the path: native_path()
+LIBRARIES["native"] = (None, [NATIVE_SOURCE], [], ["msa_b200.h", "msa_b200_lm.h"])      # the path: native_path()
 
 
 def native_path() -> str:

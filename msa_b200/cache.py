@@ -210,6 +210,10 @@ class SequenceStateCache(SparseCache):
         copied.  All int32 on the cache's device; 1 to 32 beams.  Runs in the current stream, nothing is read back; the bookkeeping
         by sequence (``slot(seq)``) stays as it was."""
         from . import _cabi_lm as A
+        if self.device.type == "cuda":
+            done = A.native().reorder(slot, parent, length, shared, self._state_parts(), self.n_slots, 32)
+            if A.count(done):
+                return done
         A.need_cuda(slot, parent, length, shared)
         if slot.dim() != 2 or not 1 <= slot.shape[1] <= 32:
             raise A.MsaError(f"reorder: slots [batch, 1 to 32 beams] expected, not {tuple(slot.shape)}")

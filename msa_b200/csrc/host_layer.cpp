@@ -11,6 +11,10 @@
 // Nothing is kept between calls.  `layers` reads the modules anew each time and answers None where anything is not what it steps
 // over: another class, a hook, a forward of its own, a bias, a subclass of Tensor, another device or type; every other function
 // answers None for operands that it does not take.  The caller then goes the way through the modules.
+//
+// The layered decoders' calls of a few microseconds are here too (the last part): from Python, the allocation of their results, the
+// tables' views and the conversion of some twenty arguments took longer than the kernels (choice of beams for one question: 28 us a call
+// for 9 us of kernels; from here 10).
 #include <dlfcn.h>
 
 #include <ATen/PythonTorchFunctionTLS.h>
@@ -23,6 +27,7 @@
 #include <array>
 
 #include "../../include/msa_b200.h"
+#include "../../include/msa_b200_lm.h"
 
 namespace {
 
@@ -315,6 +320,180 @@ py::object decode(const py::object& q_, const py::object& k_, const py::object& 
   return py::make_tuple(r[0], r[1], r[2]);
 }
 
+// ---- calls of the layered decoders
+#define MSA_LM_FUNCTIONS(F) \
+  F(msa_last_error) F(msa_lm_beam_topk_workspace) F(msa_lm_beam_topk) F(msa_lm_reorder_workspace) F(msa_lm_reorder) F(msa_lm_window_attn_tc_first) \
+  F(msa_lm_group_decode_first)
+struct LmLibrary {
+#define MSA_MEMBER(name) decltype(&::name) name = nullptr;
+  MSA_LM_FUNCTIONS(MSA_MEMBER)
+#undef MSA_MEMBER
+} lm;
+
+void bind_lm(const std::string& path) {
+  void* h = dlopen(path.c_str(), RTLD_NOW | RTLD_LOCAL);
+  TORCH_CHECK(h, "cannot load ", path, ": ", dlerror());
+  LmLibrary l;
+#define MSA_LOAD(name)                                              \
+  l.name = reinterpret_cast<decltype(l.name)>(dlsym(h, #name));     \
+  TORCH_CHECK(l.name, path, " lacks " #name);
+  MSA_LM_FUNCTIONS(MSA_LOAD)
+#undef MSA_LOAD
+  lm = l;
+}
+void check_lm(int rc, const char* what) { TORCH_CHECK(rc == 0, what, " failed (", rc, "): ", lm.msa_last_error()); }
+bool unwatched() { return !c10::impl::dispatch_mode_enabled() && !at::impl::torch_function_mode_enabled() && lm.msa_last_error; }
+bool is(const Tensor& t, at::ScalarType type, int64_t dim, c10::Device device) {
+  return t.defined() && plain_key_set(t) && t.scalar_type() == type && t.dim() == dim && t.device() == device;
+}
+bool int_table(const Tensor& t, int64_t dim, c10::Device device) { return is(t, at::kInt, dim, device) && t.is_contiguous(); }
+// An optional operand: None, or a tensor that `fits`.
+template <typename F> bool optional(const py::handle& o, Tensor& t, const F& fits) { return o.is_none() || fits(t = tensor_of(o)); }
+template <typename T> T* data(const Tensor& t) { return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr; }
+void* stream_of(c10::Device device) { return c10::cuda::getCurrentCUDAStream(device.index()).stream(); }
+Tensor bytes(int64_t n, c10::Device device) { return at::empty({n}, at::TensorOptions().dtype(at::kByte).device(device)); }
+// 32-bit numbers of `base` from `offset` on as a tensor of its own.
+Tensor table(const Tensor& base, int64_t offset, at::IntArrayRef sizes, at::ScalarType type) {
+  Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(base.storage()), base.key_set(), c10::scalarTypeToTypeMeta(type));
+  t.unsafeGetTensorImpl()->set_storage_offset(offset);
+  t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+  return t;
+}
+
+// `lm_ops.beam_topk`
+py::object beam_topk(const py::handle& logits_, const py::handle& scores_, int64_t k, const py::handle& stop_, int64_t most_beams, int64_t most_k) {
+  const Tensor logits = tensor_of(logits_), scores = tensor_of(scores_);
+  Tensor stop;
+  if (!unwatched() || !logits.defined() || !logits.is_cuda()) return py::none();
+  const c10::Device device = logits.device();
+  const bool wide = logits.scalar_type() == at::kFloat;
+  if (!is(logits, wide ? at::kFloat : at::kBFloat16, 2, device) || !is(scores, at::kFloat, 2, device) || !scores.is_contiguous() ||
+      !optional(stop_, stop, [&](const Tensor& t) { return int_table(t, 1, device); }))
+    return py::none();
+  const int64_t batch = scores.size(0), beams = scores.size(1), vocab = logits.size(1);
+  if (batch < 1 || beams < 1 || beams > most_beams || vocab < 1 || vocab > 0x7fffffff || batch * beams > 0x7fffffff || logits.size(0) != batch * beams ||
+      (vocab > 1 && logits.stride(1) != 1) || k < 1 || k > most_k || k > beams * vocab)
+    return py::none();
+  const bool live = stop.defined();
+  const int64_t n = batch * k, m = live ? batch * beams : 0;
+  Tensor out[6];
+  unlocked([&] {
+    const c10::cuda::CUDAGuard guard(device);
+    const Tensor all = at::empty({3 * (n + m)}, at::TensorOptions().dtype(at::kInt).device(device));
+    for (int i = 0; i < (live ? 6 : 3); ++i)
+      out[i] = table(all, i < 3 ? i * n : 3 * n + (i - 3) * m, {batch, i < 3 ? k : beams}, i % 3 == 0 ? at::kFloat : at::kInt);
+    const Tensor work = bytes(lm.msa_lm_beam_topk_workspace((int32_t)batch, (int32_t)beams, (int32_t)vocab, (int32_t)k), device);
+    check_lm(lm.msa_lm_beam_topk(logits.data_ptr(), logits.stride(0), wide ? MSA_F32 : MSA_BF16, scores.data_ptr<float>(), (int32_t)batch, (int32_t)beams,
+                                 (int32_t)vocab, (int32_t)k, data<int32_t>(stop), live ? (int32_t)stop.size(0) : 0, work.data_ptr(), data<float>(out[0]),
+                                 data<int32_t>(out[1]), data<int32_t>(out[2]), data<float>(out[3]), data<int32_t>(out[4]), data<int32_t>(out[5]),
+                                 stream_of(device)),
+             "msa_lm_beam_topk");
+    return 0;
+  });
+  if (!live) return py::make_tuple(out[0], out[1], out[2]);
+  return py::make_tuple(out[0], out[1], out[2], out[3], out[4], out[5]);
+}
+
+// `SequenceStateCache.reorder`; `parts`: its table of what a slot holds
+py::object reorder(const py::handle& slot_, const py::handle& parent_, const py::handle& length_, const py::handle& shared_, const py::handle& parts_,
+                   int64_t n_slots, int64_t most_beams) {
+  const Tensor slot = tensor_of(slot_), parent = tensor_of(parent_), length = tensor_of(length_), parts = tensor_of(parts_);
+  Tensor shared;
+  if (!unwatched() || !parts.defined() || !parts.is_cuda()) return py::none();
+  const c10::Device device = parts.device();
+  if (!int_table(slot, 2, device) || !int_table(parent, 2, device) || !int_table(length, 1, device) ||
+      !optional(shared_, shared, [&](const Tensor& t) { return int_table(t, 3, device); }))
+    return py::none();
+  const int64_t batch = slot.size(0), beams = slot.size(1), n_part = parts.size(0);
+  if (batch < 1 || batch > 0x7fffffff || beams < 1 || beams > most_beams || parent.sizes() != slot.sizes() || length.size(0) != batch ||
+      (shared.defined() && (shared.size(0) != batch || shared.size(1) != beams || shared.size(2) != beams)))
+    return py::none();
+  Tensor slot_out, shared_out;
+  unlocked([&] {
+    const c10::cuda::CUDAGuard guard(device);
+    const auto ints = at::TensorOptions().dtype(at::kInt).device(device);
+    slot_out = at::empty({batch, beams}, ints);
+    if (shared.defined()) shared_out = at::empty({batch, beams, beams}, ints);
+    const Tensor work = bytes(lm.msa_lm_reorder_workspace((int32_t)batch, (int32_t)beams, (int32_t)n_part), device);
+    check_lm(lm.msa_lm_reorder(data<int32_t>(slot), data<int32_t>(parent), data<int32_t>(length), data<int32_t>(shared), (int32_t)batch, (int32_t)beams,
+                               (int32_t)n_slots, static_cast<const msa_lm_state_part*>(parts.data_ptr()), (int32_t)n_part, data<int32_t>(slot_out),
+                               data<int32_t>(shared_out), work.data_ptr(), stream_of(device)),
+             "msa_lm_reorder");
+    return 0;
+  });
+  if (!shared_out.defined()) return py::make_tuple(slot_out, py::none());
+  return py::make_tuple(slot_out, shared_out);
+}
+
+// `lm_ops.window_attn_tc` without rotated parts
+bool window_attn_tc(const py::handle& q_, const py::handle& k_, const py::handle& v_, const py::handle& out_, const py::handle& gate_, const py::handle& start_,
+                    const py::handle& cu_, const py::handle& ctx_off_, const py::handle& status_, double scale, int64_t window, int64_t first, bool sink,
+                    int64_t seq0, int64_t seq1, int64_t max_len, int64_t row0) {
+  const Tensor q = tensor_of(q_), k = tensor_of(k_), v = tensor_of(v_), out = tensor_of(out_), start = tensor_of(start_), cu = tensor_of(cu_),
+               ctx_off = tensor_of(ctx_off_), status = tensor_of(status_);
+  Tensor gate;
+  if (!unwatched() || !q.defined() || !q.is_cuda()) return false;
+  const c10::Device device = q.device();
+  for (const Tensor* t : {&q, &k, &v, &out})
+    if (!is(*t, at::kBFloat16, 3, device) || t->stride(2) != 1 || t->size(0) > 0x7fffffff) return false;
+  for (const Tensor* t : {&start, &cu, &ctx_off, &status})
+    if (!int_table(*t, 1, device)) return false;
+  if (!optional(gate_, gate, [&](const Tensor& t) { return is(t, at::kBFloat16, 2, device) && t.stride(1) == 1 && t.size(0) == q.size(0) && t.size(1) == q.size(1); }))
+    return false;
+  const int64_t k_heads = k.size(1), v_heads = v.size(1), kv = std::max(k_heads, v_heads);
+  if (kv < 1 || q.size(1) < 1) return false;
+  msa_lm_attn_args a{};
+  a.qa = q.data_ptr(); a.qa_row = q.stride(0); a.qa_head = q.stride(1);
+  a.ka = k.data_ptr(); a.ka_row = k.stride(0); a.ka_head = k_heads == 1 ? 0 : k.stride(1);
+  a.v = v.data_ptr(); a.v_row = v.stride(0); a.v_head = v_heads == 1 ? 0 : v.stride(1);
+  a.out = out.data_ptr(); a.out_row = out.stride(0); a.out_head = out.stride(1);
+  a.gate = data<void>(gate); a.gate_row = gate.defined() ? gate.stride(0) : 0;
+  a.start = data<int32_t>(start); a.cu = data<int32_t>(cu); a.ctx_off = data<int32_t>(ctx_off);
+  a.group = (int32_t)(q.size(1) / kv); a.sink = sink; a.seq0 = (int32_t)seq0; a.seq1 = (int32_t)seq1; a.max_len = (int32_t)max_len;
+  a.heads = (int32_t)q.size(1); a.da = (int32_t)q.size(2); a.dv = (int32_t)v.size(2); a.window = (int32_t)window;
+  a.qa_dtype = a.out_dtype = a.dtype = MSA_BF16; a.scale = (float)scale;
+  unlocked([&] {
+    const c10::cuda::CUDAGuard guard(device);
+    check_lm(lm.msa_lm_window_attn_tc_first(&a, (int32_t)first, (int32_t)q.size(0), (int32_t)k.size(0), (int32_t)row0, data<int32_t>(status), stream_of(device)),
+             "msa_lm_window_attn_tc_first");
+    return 0;
+  });
+  return true;
+}
+
+// `lm_ops.group_decode`; `merge`: the splits are joined by a kernel of their own
+bool group_decode(const py::handle& q_, const py::handle& ring_, const py::handle& slot_, const py::handle& pos_, const py::handle& out_, const py::handle& gate_,
+                  int64_t kv_heads, int64_t window, int64_t first, double scale, bool sink, int64_t splits, bool merge) {
+  const Tensor q = tensor_of(q_), ring = tensor_of(ring_), slot = tensor_of(slot_), pos = tensor_of(pos_), out = tensor_of(out_);
+  Tensor gate;
+  if (!unwatched() || !q.defined() || !q.is_cuda()) return false;
+  const c10::Device device = q.device();
+  const int64_t n = is(q, at::kBFloat16, 3, device) ? q.size(0) : 0;
+  if (n < 1 || !is(out, at::kBFloat16, 3, device) || !is(ring, at::kBFloat16, 3, device) || !ring.is_contiguous() || !int_table(slot, 1, device) ||
+      !int_table(pos, 1, device) || slot.size(0) < n || pos.size(0) < n || out.size(0) != n || out.size(1) != q.size(1) ||
+      !optional(gate_, gate, [&](const Tensor& t) { return is(t, at::kBFloat16, 2, device) && t.stride(1) == 1 && t.size(0) == n && t.size(1) == q.size(1); }))
+    return false;
+  const int64_t heads = q.size(1), dim = q.size(2), vdim = out.size(2);
+  if (q.stride(2) != 1 || q.stride(1) != dim || out.stride(2) != 1 || out.stride(1) != vdim || ring.size(2) != kv_heads * (dim + vdim)) return false;
+  unlocked([&] {
+    const c10::cuda::CUDAGuard guard(device);
+    Tensor work;
+    float *part_o = nullptr, *part_ml = nullptr;
+    if (merge) {                                    // one allocation for both
+      work = bytes(n * heads * splits * (vdim + 2) * 4, device);
+      part_o = static_cast<float*>(work.data_ptr());
+      part_ml = part_o + n * heads * splits * vdim;
+    }
+    check_lm(lm.msa_lm_group_decode_first(q.data_ptr(), q.stride(0), ring.data_ptr(), ring.size(1), data<int32_t>(slot), data<int32_t>(pos), (int32_t)n,
+                                          (int32_t)heads, (int32_t)kv_heads, (int32_t)dim, (int32_t)vdim, (int32_t)window, (int32_t)first, (int32_t)splits,
+                                          (float)scale, sink, data<void>(gate), gate.defined() ? gate.stride(0) : 0, out.data_ptr(), out.stride(0), part_o,
+                                          part_ml, stream_of(device)),
+             "msa_lm_group_decode_first");
+    return 0;
+  });
+  return true;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_native, m) {
@@ -329,4 +508,9 @@ PYBIND11_MODULE(_native, m) {
   m.def("back", &back);
   m.def("angles", &angles);
   m.def("decode", &decode);
+  m.def("bind_lm", &bind_lm);
+  m.def("beam_topk", &beam_topk);
+  m.def("reorder", &reorder);
+  m.def("window_attn_tc", &window_attn_tc);
+  m.def("group_decode", &group_decode);
 }

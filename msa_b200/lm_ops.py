@@ -172,6 +172,9 @@ def beam_topk(logits: torch.Tensor, scores: torch.Tensor, k: int, stop: Optional
 
     With ``stop`` (int32 token ids, may be empty) three more, ``[batch, beams]``: the first ``beams`` of the k whose token is not
     among them, which are the next beams (``k >= beams * (1 + len(stop))`` always finds that many, where there are that many)."""
+    done = A.native().beam_topk(logits, scores, k, stop, BEAM_MAX, BEAM_MAX_K)
+    if A.count(done):
+        return done
     A.need_cuda(logits, scores, stop)
     if logits.dim() != 2 or scores.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16) or scores.dtype != torch.float32:
         raise A.MsaError("beam_topk: fp32 or bf16 logits [batch * beams, vocab] and fp32 scores [batch, beams] expected")
@@ -274,8 +277,15 @@ def window_attn_tc_supported(dim, rot, vdim, dtype, scale) -> bool:
     return dtype == torch.bfloat16 and scale > 0 and bool(A.lib().msa_lm_window_attn_tc_supported(dim, rot, vdim))
 
 
+def _native_window(q, k, v, out, row0, status, first, *, scale, window, start, cu, seq0, seq1, max_len, ctx_off=None, sink=False, gate=None, **more):
+    """Whether the call was made from native code, which takes neither slots nor rings."""
+    return not more and A.native().window_attn_tc(q, k, v, out, gate, start, cu, ctx_off, status, scale, window, first, bool(sink), seq0, seq1, max_len, row0)
+
+
 def window_attn_tc(qa, qb, ka, kb, v, out, *, row0, status, first=0, **kw):
     """The portions of a step on the tensor cores: ``qa`` / ``out`` from the first portion row (packed row ``row0``) on."""
+    if qb is None and kb is None and A.count(_native_window(qa, ka, v, out, row0, status, first, **kw)):
+        return
     args = attn_args(qa, qb, ka, kb, v, out, **kw)
     A.call("msa_lm_window_attn_tc_first", C.byref(args), first, qa.shape[0], ka.shape[0], row0, A.ptr(status), A.stream_ptr(qa.device))
 
@@ -352,9 +362,12 @@ def group_decode(q, ring, kv_heads, step, out, *, window, scale, sink, gate, fir
     vdim = out.shape[2]
     splits = group_decode_splits(n, heads, kv_heads, ring.shape[1])
     part_o = part_ml = 0
+    merge = splits > 1
     if first and splits_join(splits, ring.shape[1]):
-        splits = min(splits, GROUP_CLUSTER)
-    elif splits > 1:                                             # one allocation for both
+        splits, merge = min(splits, GROUP_CLUSTER), False
+    if A.count(A.native().group_decode(q, ring, step.slot, step.start, out, gate, kv_heads, window, first, scale, bool(sink), splits, merge)):
+        return
+    if merge:                                                    # one allocation for both
         work = torch.empty(n * heads * splits * (vdim + 2), dtype=torch.float32, device=q.device)
         part_o = work.data_ptr()
         part_ml = part_o + n * heads * splits * vdim * 4
