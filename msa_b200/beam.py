@@ -67,7 +67,7 @@ def advance(logits: torch.Tensor, searches: Sequence[Tuple[BeamSearch, Sequence[
         rows = [r for i in members for r in (list(searches[i][1]) * beams)[:beams]]
         if rows == list(range(rows[0], rows[0] + len(rows))):
             x = logits[rows[0]:rows[0] + len(rows)]
-        elif len(members) == 1:
+        elif len(set(rows)) == 1:
             x = logits[rows[0]:rows[0] + 1].expand(beams, -1)
         else:
             x = logits[torch.tensor(rows, device=logits.device)]

@@ -1,8 +1,9 @@
 // Beam search: the choice of the next beams from the logits, and the reordering of the sequence states that follows from it.
 //
 // Choice.  A candidate (beam b, token t) has the score  s_b + (x_bt - lse_b),  lse_b = log sum_t exp x_bt.  Within a row the order is
-// that of the logits, so one pass over a row yields both its sum and its k best logits; the second kernel joins a question's rows in
-// 64 bits.  Bound by the one read of the logits.
+// that of the logits, so one pass over a row yields its sum and the largest logit of every 512, and a question's k best lie in the k chunks
+// whose largest are the best; the second kernel ranks those, reads them again and ranks what lies in them, in 64 bits.  Bound by the one read
+// of the logits (48 x 4 rows of 151,936 fp32: 23 us at 5.1 TB/s, then 8), for few rows by the second kernel's chain of barriers (7 us).
 //
 // Reordering.  New beam j continues beam parent[j].  Its first child keeps a beam's slot, the others take slots that nobody
 // continues: sources and destinations never meet, and no second buffer is needed.  Bound by the copied bytes, read and written once.
