@@ -235,3 +235,19 @@ def test_engine_refuses_beams_over_a_memory(tmp_path):
     (tmp_path / "config.json").write_text(json.dumps({"architectures": ["MSAForCausalLM"], "msa_config": {}}))
     with pytest.raises(ValueError, match="num_beams"):
         MSAEngine(GenerateConfig(devices=[0], num_beams=2), ModelConfig(model_path=str(tmp_path)), start=False)
+
+
+@pytest.mark.parametrize("rows,want", [([4], [4, 4, 4]), ([2, 3, 4], [2, 3, 4]), ([5, 1, 3], [5, 1, 3])])
+def test_a_search_chooses_from_its_own_rows(rows, want, monkeypatch):
+    """One row behind the prompt stands for every beam; later rows lie wherever the step put them."""
+    from msa_b200 import beam
+    seen = []
+
+    def choose(x, scores, k, stop):
+        seen.append(x.clone())
+        table = lambda n: (torch.zeros((1, n)), torch.zeros((1, n), dtype=torch.int32), torch.zeros((1, n), dtype=torch.int32))
+        return table(k) + table(3)
+    monkeypatch.setattr(beam.K, "beam_topk", choose)
+    logits = torch.arange(6.0)[:, None].expand(6, 8).contiguous()
+    assert beam.advance(logits, [(beam.BeamSearch(3, 10), rows)]) == [False]
+    assert seen[0][:, 0].tolist() == want
