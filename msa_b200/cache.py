@@ -235,7 +235,8 @@ class SequenceStateCache(SparseCache):
     def reorder_beams(self, groups: Sequence[Sequence[Hashable]], parents: Sequence[Sequence[int]]) -> None:
         """``reorder`` by sequence: ``groups[q]`` are the sequences of question q's beams (as many for every question), and beam j goes on from
         beam ``parents[q][j]``, or from nobody (-1).  Beams that others go on from hold equally many positions; afterwards all of the
-        question do, and ``slot`` and ``length`` say where and how many.  One copy of tables to the device, no read-back."""
+        question do, and ``slot`` and ``length`` say where and how many.  Which rows beams have in common is remembered for the group as it
+        stands here, until a call names one of its sequences in another group.  One copy of tables to the device, no read-back."""
         groups, parents = [tuple(g) for g in groups], [list(p) for p in parents]
         if not groups:
             return
@@ -273,6 +274,10 @@ class SequenceStateCache(SparseCache):
             flat, b = flat.to(self.device, non_blocking=True), len(groups)
             slot, parent, length, shared = flat.split([b * beams, b * beams, b, b * beams * beams])
             self.reorder(slot.view(b, beams), parent.view(b, beams), length, shared.view(b, beams, beams))
+        # A table counts for its own group alone: what another one says of these sequences is over.
+        moved, named = set(groups), set(seqs)
+        for g in [g for g in self._shared if g not in moved and not named.isdisjoint(g)]:
+            del self._shared[g]
         for g, held, (own, n, table) in zip(groups, slots, new):
             for s, o in zip(g, own):
                 self._slot[s], self._length[s] = held[o], n
