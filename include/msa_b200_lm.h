@@ -347,7 +347,8 @@ typedef struct {
  * first that names a parent keeps its slot, the others (and those with a parent outside 0 .. beams-1, which get no state) take, in
  * order, the slots of beams that nobody names.  slot_out [batch, beams]: the new table.  parts [n_part] (device memory): the
  * tensors.  shared [batch, beams, beams] (may be null): positions from the start on whose ring rows two beams' slots hold alike;
- * those are not copied; shared_out the same for the new beams.  slot: distinct, below n_slots (a copy to or from others is left out).
+ * those are not copied; shared_out the same for the new beams.  Slots that hold other numbers of positions than length[q], longer ones among
+ * them, have nothing in common with the others: 0.  slot: distinct, below n_slots (a copy to or from others is left out).
  * workspace: msa_lm_reorder_workspace bytes, 16-byte aligned. */
 int64_t msa_lm_reorder_workspace(int32_t batch, int32_t beams, int32_t n_part);
 int msa_lm_reorder(const int32_t* slot, const int32_t* parent, const int32_t* length, const int32_t* shared, int32_t batch, int32_t beams,

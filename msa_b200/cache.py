@@ -206,8 +206,8 @@ class SequenceStateCache(SparseCache):
         first beam that names a parent keeps its slot; the others take, in order, the slots that nobody continues, and the parent's
         state is copied there, in every run.  A parent of -1 names nobody: such a beam gets a slot, but no state.  ``shared``
         ``[batch, beams, beams]``: positions from the start on whose ring rows two beams' slots hold alike (zeros when beams begin,
-        then what the last call returned, as long as the slots advance by nothing but the beams' own tokens); those rows are not
-        copied.  All int32 on the cache's device; 1 to 32 beams.  Runs in the current stream, nothing is read back; the bookkeeping
+        then what the last call returned, as long as the slots advance by nothing but the beams' own tokens, and all by as many); those
+        rows are not copied.  All int32 on the cache's device; 1 to 32 beams.  Runs in the current stream, nothing is read back; the bookkeeping
         by sequence (``slot(seq)``) stays as it was."""
         from . import _cabi_lm as A
         if self.device.type == "cuda":
@@ -259,7 +259,11 @@ class SequenceStateCache(SparseCache):
             for x in p:                                             # what the kernel does with the slots
                 own.append(x if x >= 0 and x not in taken else spare.pop(0))
                 taken.add(x)
+            # A slot that holds another number of positions than the parents' has other rows in its rings: nothing in common counts.
+            alike = [self._length[s] == n for s in g]
             start = self._shared.get(g) or [[0] * beams for _ in range(beams)]
+            if not all(alike):
+                start = [[x if i and j else 0 for x, j in zip(row, alike)] for row, i in zip(start, alike)]
             origin = [x if x >= 0 else o for x, o in zip(p, own)]
             table = [[n if a == b else start[a][b] for b in origin] for a in origin]
             slots.append([self._slot[s] for s in g])

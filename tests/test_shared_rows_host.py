@@ -121,3 +121,48 @@ def test_only_what_a_call_names_is_forgotten():
     m.move(("ab", [0, 0]), ("cd", [0, 0]), ("ef", [0, 0]))
     m.move(("bc", [-1, 1]), ("ef", [1, 0]))
     assert set(m.cache._shared) == {("b", "c"), ("e", "f")} and m.cache._shared["e", "f"] == [[5, 5], [5, 5]]
+
+
+@pytest.mark.parametrize("ahead", [3, 15, 30])
+def test_a_beam_that_nobody_goes_on_from_is_ahead(ahead):
+    """Its ring has written over rows that both had in common."""
+    m = Lives("ab", [RingSpec(1, 16), RingSpec(1, 4, first=2), RingSpec(1, None)])
+    m.grow(a=20)
+    m.move(("ab", [0, 0]))
+    m.grow(a=1, b=ahead)
+    m.move(("ab", [0, 0]))
+
+
+@pytest.mark.parametrize("lead", [-7, 9, 25])
+def test_a_beam_of_another_length_is_left_and_then_taken(lead):
+    """b goes on from nobody, its length becomes the question's, and only the step after that copies into its slot."""
+    m = Lives("abc")
+    m.grow(a=20)
+    m.move(("abc", [0, 0, 0]))
+    m.grow(a=max(1, 1 - lead), c=max(1, 1 - lead), b=max(1, 1 + lead))
+    m.move(("abc", [0, -1, 2]))
+    m.grow(a=1, b=1, c=1)
+    m.move(("abc", [0, 2, 0]))
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_lives_of_every_kind(seed):
+    """Groups of any members in any order, lengths that part and meet, beams that nobody goes on from."""
+    import random
+    rng = random.Random(seed)
+    m = Lives("abcdef", [RingSpec(1, 7, first=3), RingSpec(1, 11), RingSpec(1, None)])
+    m.grow(**{s: rng.randint(0, 9) for s in "abcdef"})
+    groups = ["abc", "de", "f"]
+    for _ in range(30):
+        if rng.random() < 0.15:
+            names, size = rng.sample("abcdef", 6), rng.randint(1, 3)
+            groups = ["".join(names[at:at + size]) for at in range(0, 7 - size, size)]
+        pairs = []
+        for g in groups:
+            n = m.cache.length(rng.choice(g))
+            from_ = [i for i, s in enumerate(g) if m.said[s] is not None and m.cache.length(s) == n]
+            pairs.append((g, [rng.choice(from_) if from_ and rng.random() < 0.8 else -1 for _ in g]))
+        for size in {len(g) for g in groups}:
+            m.move(*[p for p in pairs if len(p[0]) == size])
+        one = rng.randint(0, 4)
+        m.grow(**{s: one if rng.random() < 0.8 else rng.randint(0, 14) for s in "abcdef"})
