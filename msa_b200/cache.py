@@ -208,8 +208,10 @@ class SequenceStateCache(SparseCache):
         ``[batch, beams, beams]``: positions from the start on whose ring rows two beams' slots hold alike (zeros when beams begin,
         then what the last call returned, as long as the slots advance by nothing but the beams' own tokens, and all by as many); those
         rows are not copied.  All int32 on the cache's device; 1 to 32 beams.  Runs in the current stream, nothing is read back; the bookkeeping
-        by sequence (``slot(seq)``) stays as it was."""
+        by sequence (``slot(seq)``) stays as it was, and what ``reorder_beams`` remembers is forgotten (a captured call does so when it is
+        captured: its replays are not for slots that ``reorder_beams`` moves, too)."""
         from . import _cabi_lm as A
+        self._shared.clear()                 # whose slots these are is on the device: nothing that is known by sequence counts from here on
         if self.device.type == "cuda":
             done = A.native().reorder(slot, parent, length, shared, self._state_parts(), self.n_slots, 32)
             if A.count(done):
@@ -270,6 +272,9 @@ class SequenceStateCache(SparseCache):
             lengths.append(n)
             tables.append(start)
             new.append((own, n, table))
+        # A table counts for its own group alone: what another one says of these sequences is over.
+        named = set(seqs)
+        others = {g: table for g, table in self._shared.items() if named.isdisjoint(g)}
         if any(x != j for p in parents for j, x in enumerate(p)):   # else nobody moves
             flat = torch.tensor([x for t in (slots, parents) for row in t for x in row] + lengths + [x for t in tables for row in t for x in row],
                                 dtype=torch.int32)
@@ -278,10 +283,7 @@ class SequenceStateCache(SparseCache):
             flat, b = flat.to(self.device, non_blocking=True), len(groups)
             slot, parent, length, shared = flat.split([b * beams, b * beams, b, b * beams * beams])
             self.reorder(slot.view(b, beams), parent.view(b, beams), length, shared.view(b, beams, beams))
-        # A table counts for its own group alone: what another one says of these sequences is over.
-        moved, named = set(groups), set(seqs)
-        for g in [g for g in self._shared if g not in moved and not named.isdisjoint(g)]:
-            del self._shared[g]
+        self._shared = others
         for g, held, (own, n, table) in zip(groups, slots, new):
             for s, o in zip(g, own):
                 self._slot[s], self._length[s] = held[o], n

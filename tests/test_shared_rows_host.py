@@ -166,3 +166,23 @@ def test_lives_of_every_kind(seed):
             m.move(*[p for p in pairs if len(p[0]) == size])
         one = rng.randint(0, 4)
         m.grow(**{s: one if rng.random() < 0.8 else rng.randint(0, 14) for s in "abcdef"})
+
+
+def test_tables_moved_by_hand(monkeypatch):
+    """`reorder` itself, whose slots only the device knows: nothing that was known by sequence counts behind it."""
+    import contextlib
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from msa_b200 import _cabi_lm as A
+    monkeypatch.undo()
+    seen = []
+    monkeypatch.setattr(A, "call", lambda name, *a: seen.append(name))
+    monkeypatch.setattr(A, "stream_ptr", lambda device=None: 0)
+    monkeypatch.setattr(A, "ptr", lambda t: 0)
+    monkeypatch.setattr(A, "on_device", lambda d: contextlib.nullcontext())
+    monkeypatch.setattr(SequenceStateCache, "_state_parts", lambda self: torch.empty((2, 6), dtype=torch.int64))
+    with FakeTensorMode():
+        c = SequenceStateCache([RingSpec(6, 8)], 4, 50, "cuda:0", torch.float32)
+        c._shared["a", "b"] = [[3, 3], [3, 3]]
+        t = torch.empty((1, 2), dtype=torch.int32, device="cuda:0")
+        c.reorder(t, t, t[0, :1])
+    assert seen == ["msa_lm_reorder"] and not c._shared
