@@ -53,8 +53,29 @@ class BeamSearch:
 
     @property
     def choices(self) -> int:
-        """Continuations to ask for: enough for ``beams`` that do not end, if ``beam_topk`` gives that many."""
+        """Continuations to ask for: enough for ``beams`` that do not end, if ``beam_topk`` gives that many (``choose`` sees to it
+        that no more are needed)."""
         return min(K.BEAM_MAX_K, self.beams * (1 + len(self.stop)))
+
+
+def choose(x: torch.Tensor, scores: torch.Tensor, k: int, stop: Sequence[int]):
+    """``beam_topk`` of the ``k`` best, of which ``beams`` go on whatever the others are: stop tokens take at most ``len(stop)`` places a
+    beam.  Where that is more than ``beam_topk`` gives, the best are chosen by themselves, and for the beams that go on a row's stop
+    tokens are one of their joint probability: log softmax stays what it was (but for the rounding of that one logit), and one place
+    a beam is enough."""
+    beams, vocab = scores.shape[1], x.shape[1]
+    ids = lambda tokens: torch.tensor(tokens, dtype=torch.int32, device=x.device)
+    if k >= min(beams * (1 + len(stop)), beams * vocab):
+        return K.beam_topk(x, scores, k, ids(stop))
+    known = [t for t in stop if 0 <= t < vocab]
+    one = x.float()
+    if len(known) > 1:
+        at = ids(known).long()
+        joint = torch.logsumexp(one[:, at], 1)
+        one = one.index_fill(1, at, -math.inf)
+        one[:, known[0]] = joint
+    live = K.beam_topk(one, scores, min(2 * beams, beams * vocab), ids(known[:1]))[3:]
+    return (*K.beam_topk(x, scores, min(beams, k)), *live)
 
 
 def advance(logits: torch.Tensor, searches: Sequence[Tuple[BeamSearch, Sequence[int]]]) -> List[bool]:
@@ -72,7 +93,7 @@ def advance(logits: torch.Tensor, searches: Sequence[Tuple[BeamSearch, Sequence[
         else:
             x = logits[torch.tensor(rows, device=logits.device)]
         scores = torch.tensor([searches[i][0].scores for i in members], dtype=torch.float32).to(logits.device)
-        out = K.beam_topk(x, scores, min(k, beams * x.shape[1]), torch.tensor(stop, dtype=torch.int32, device=logits.device))
+        out = choose(x, scores, min(k, beams * x.shape[1]), stop)
         flat = torch.cat([t.view(torch.int32) for t in out], dim=1).cpu()          # one copy to the host
         parts = flat.split([t.shape[1] for t in out], dim=1)
         lists = [p.contiguous().view(torch.float32).tolist() if j % 3 == 0 else p.tolist() for j, p in enumerate(parts)]
