@@ -36,7 +36,7 @@ class BeamSearch:
         """``candidates`` and ``live``: (score, beam, token) lists as ``beam_topk`` returns them.  True when the search is over; else
         ``parents`` and ``next_tokens`` say how the beams go on."""
         for score, beam, token in candidates[:self.beams]:
-            if token in self.stop:
+            if beam >= 0 and token in self.stop:                            # -1: a place without a continuation
                 self._end(score, self.tokens[beam] + [token])
         self.parents = [beam for _, beam, _ in live]
         self.next_tokens = [max(token, 0) for _, _, token in live]          # beams that are gone run along with any token

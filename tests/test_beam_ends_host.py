@@ -82,3 +82,12 @@ def test_rows_of_a_kind(kind):
 
 def search_scores(beams):
     return torch.tensor([-0.1 * i for i in range(beams)], dtype=torch.float32).tolist()
+
+
+def test_places_without_a_continuation_do_not_end():
+    """-1, which some tokenizers have for no end token, is what stands in places left over."""
+    inf = math.inf
+    s = B.BeamSearch(3, 5, stop=[-1, 2])
+    left = (-inf, -1, -1)
+    assert not s.update([(-1.0, 0, 1), left, left], [(-1.0, 0, 1), left, left]) and s.ended == []
+    assert s.update([(-1.5, 0, 2), left, left], [left, left, left]) and s.ended == [(-0.75, [1, 2])]
