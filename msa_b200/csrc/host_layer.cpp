@@ -53,7 +53,19 @@ void bind(const std::string& path) {
 #undef MSA_LOAD
   lib = l;
 }
-void check(int rc, const char* what) { TORCH_CHECK(rc == 0, what, " failed (", rc, "): ", lib.msa_last_error()); }
+// What a function of the libraries refuses: `MsaError` to Python, in the words of the calls that Python makes itself.
+struct Refused : std::runtime_error { using std::runtime_error::runtime_error; };
+void check_call(int rc, const char* what, const char* (*last_error)()) {
+  if (rc != 0) throw Refused(std::string(what) + " failed (" + std::to_string(rc) + "): " + last_error());
+}
+void raise_refused(std::exception_ptr p) {
+  try {
+    if (p) std::rethrow_exception(p);
+  } catch (const Refused& e) {
+    py::set_error(py::module_::import("msa_b200._cabi").attr("MsaError"), e.what());
+  }
+}
+void check(int rc, const char* what) { check_call(rc, what, lib.msa_last_error); }
 
 // ---- what the fused calls take
 bool plain_key_set(const Tensor& t) {             // no wrapper of a transformation, no negative or conjugate view
@@ -341,7 +353,7 @@ void bind_lm(const std::string& path) {
 #undef MSA_LOAD
   lm = l;
 }
-void check_lm(int rc, const char* what) { TORCH_CHECK(rc == 0, what, " failed (", rc, "): ", lm.msa_last_error()); }
+void check_lm(int rc, const char* what) { check_call(rc, what, lm.msa_last_error); }
 bool unwatched() { return !c10::impl::dispatch_mode_enabled() && !at::impl::torch_function_mode_enabled() && lm.msa_last_error; }
 bool is(const Tensor& t, at::ScalarType type, int64_t dim, c10::Device device) {
   return t.defined() && plain_key_set(t) && t.scalar_type() == type && t.dim() == dim && t.device() == device;
@@ -497,6 +509,7 @@ bool group_decode(const py::handle& q_, const py::handle& ring_, const py::handl
 }  // namespace
 
 PYBIND11_MODULE(_native, m) {
+  py::register_local_exception_translator(&raise_refused);
   tensor_type = reinterpret_cast<PyTypeObject*>(THPVariableClass);
   py::object parameter = py::module_::import("torch.nn.parameter").attr("Parameter");
   parameter_type = reinterpret_cast<PyTypeObject*>(parameter.release().ptr());
