@@ -265,7 +265,7 @@ def attn_args(qa, qb, ka, kb, v, out, *, scale, window, start, cu, seq0, seq1, m
         qa.data_ptr(), q_row, q_head, qb_ptr, qb_row, qb_head, ka.data_ptr(), k_row, 0 if k_heads == 1 else k_head, kb_ptr, kb_row, kb_head,
         v.data_ptr(), v_row, 0 if v_heads == 1 else v_head, out.data_ptr(), o_row, o_head, ptr(gate), 0 if gate is None else gate.stride(0),
         ptr(slot), ptr(start), ptr(cu), ptr(ctx_off), ring_rows, heads // max(k_heads, v_heads), 1 if sink else 0, seq0, seq1, max_len,
-        heads, da, db, dv, window, A.dtype_code(qa.dtype), A.dtype_code(out.dtype), A.dtype_code(ka.dtype), float(scale))
+        heads, da, db, dv, window, A.dtype_code(qa.dtype), A.dtype_code(out.dtype), A.dtype_code(ka.dtype), scale)
 
 
 def window_attn(qa, qb, ka, kb, v, out, *, first=0, **kw):
