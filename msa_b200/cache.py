@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import os
 from dataclasses import dataclass
+from operator import is_
 from typing import Dict, Hashable, List, Optional, Sequence, Tuple
 
 import torch
@@ -140,6 +141,7 @@ class SequenceStateCache(SparseCache):
         self._length: Dict[Hashable, int] = {}
         self._shared: Dict[Tuple[Hashable, ...], List[List[int]]] = {}
         self._parts: Optional[torch.Tensor] = None
+        self._parts_of: List[torch.Tensor] = []
         if self.device.type == "cuda":
             self._state_parts()              # here, so that a first ``reorder`` may be captured
 
@@ -174,8 +176,10 @@ class SequenceStateCache(SparseCache):
         self._length[seq] += n
 
     def _state_parts(self) -> torch.Tensor:
-        """What a slot holds, tensor by tensor, for the kernels (``msa_lm_state_part``): device memory, made once."""
-        if self._parts is None:
+        """What a slot holds, tensor by tensor, for the kernels (``msa_lm_state_part``): device memory, made once, and again when another
+        tensor has taken the place of one of them."""
+        tensors = [*self.ring.values(), *self.conv.values(), *self.state.values(), *self.shift.values(), self.last_token]
+        if self._parts is None or not all(map(is_, tensors, self._parts_of)):
             from . import _cabi_lm as A
             parts = []
 
@@ -195,7 +199,7 @@ class SequenceStateCache(SparseCache):
                         add(d[i], A.STATE_ALL, d[i][0].numel() * d[i].element_size())
             add(self.last_token, A.STATE_ALL, self.last_token.element_size())
             raw = torch.frombuffer(bytearray(b"".join(bytes(p) for p in parts)), dtype=torch.int64).view(len(parts), -1)
-            self._parts = raw.to(self.device)
+            self._parts, self._parts_of = raw.to(self.device), tensors
         return self._parts
 
     def reorder(self, slot: torch.Tensor, parent: torch.Tensor, length: torch.Tensor, shared: Optional[torch.Tensor] = None
