@@ -217,7 +217,8 @@ class SequenceStateCache(SparseCache):
         from . import _cabi_lm as A
         self._shared.clear()                 # whose slots these are is on the device: nothing that is known by sequence counts from here on
         if self.device.type == "cuda":
-            done = A.native().reorder(slot, parent, length, shared, self._state_parts(), self.n_slots, 32)
+            done = A.native().reorder(slot, parent, length, shared, self._parts, self._parts_of, (self.ring, self.conv, self.state, self.shift),
+                                      self.last_token, self.n_slots, 32)
             if A.count(done):
                 return done
         A.need_cuda(slot, parent, length, shared)

@@ -406,9 +406,23 @@ py::object beam_topk(const py::handle& logits_, const py::handle& scores_, int64
   return py::make_tuple(out[0], out[1], out[2], out[3], out[4], out[5]);
 }
 
-// `SequenceStateCache.reorder`; `parts`: its table of what a slot holds
+// Whether `held` lists exactly what is in `tables`, one after the other, and `last`.
+bool lists(const py::list& held, const py::tuple& tables, const py::handle& last) {
+  Py_ssize_t n = 0;
+  const Py_ssize_t size = PyList_GET_SIZE(held.ptr());
+  for (const py::handle& table : tables) {
+    if (!PyDict_Check(table.ptr())) return false;
+    PyObject *key, *value;
+    for (Py_ssize_t at = 0; PyDict_Next(table.ptr(), &at, &key, &value); ++n)
+      if (n >= size || PyList_GET_ITEM(held.ptr(), n) != value) return false;
+  }
+  return n + 1 == size && PyList_GET_ITEM(held.ptr(), n) == last.ptr();
+}
+
+// `SequenceStateCache.reorder`; `parts`: its table of what a slot holds, made for the tensors `held`, which the cache has to hold still
 py::object reorder(const py::handle& slot_, const py::handle& parent_, const py::handle& length_, const py::handle& shared_, const py::handle& parts_,
-                   int64_t n_slots, int64_t most_beams) {
+                   const py::list& held, const py::tuple& tables, const py::handle& last, int64_t n_slots, int64_t most_beams) {
+  if (!lists(held, tables, last)) return py::none();
   const Tensor slot = tensor_of(slot_), parent = tensor_of(parent_), length = tensor_of(length_), parts = tensor_of(parts_);
   Tensor shared;
   if (!unwatched() || !parts.defined() || !parts.is_cuda()) return py::none();
