@@ -37,8 +37,8 @@ def reorder(self, slot, parent, length, shared=None):
 class Lives:
     """Sequences on rings, and what was written for each of them."""
 
-    def __init__(self, names, specs=(RingSpec(1, 16),), max_len=400):
-        self.cache = SequenceStateCache(list(specs), len(names), max_len, "cpu", torch.float32)
+    def __init__(self, names, specs=(RingSpec(1, 16),), max_len=400, device="cpu"):
+        self.cache = SequenceStateCache(list(specs), len(names), max_len, device, torch.float32)
         self.said, self.count = {s: [] for s in names}, 0
         for s in names:
             self.cache.acquire(s)
