@@ -2,8 +2,9 @@
 // plain and rotated query / key parts and values are multiples of 64 wide.
 //
 // Work item = 256 consecutive query tokens of one head: two tiles of 128 rows that share every key / value tile on its
-// way through shared memory.  One persistent CTA per SM, 320 threads: warps 0-3 the softmax of tile 0, 4-7 that of tile 1
-// (thread = query row = TMEM lane), warp 8 the TMA producer, warp 9 the MMA issuer.  Per 64-key tile and query tile:
+// way through shared memory.  One persistent CTA per SM, 352 threads: warps 0-3 the softmax of tile 0, 4-7 that of tile 1
+// (thread = query row = TMEM lane), warp 8 the TMA producer, warp 9 the MMA issuer, warp 10 clears values that are not the portion's
+// own.  Per 64-key tile and query tile:
 //     S = Q K^T    K-major operands; the key's plain part comes from the expanded keys of the head, its rotated part from
 //                  the context row all heads share; fp32 into one of two 64-column TMEM buffers of the tile;
 //     softmax      fp32, running maximum advanced only when it moved by more than 2^8; P as bf16 over the consumed columns;
@@ -17,7 +18,7 @@
 namespace msa {
 
 constexpr int kWaRows = 128, kWaTiles = 2, kWaKeys = 64;
-constexpr int kWaThreads = 32 * (4 * kWaTiles + 2);
+constexpr int kWaThreads = 32 * (4 * kWaTiles + 3);
 constexpr int kWaQBlk = kWaRows * 128;                    // one 64-column block of a query tile: 16 KB
 constexpr int kWaKBlk = kWaKeys * 128;                    // one 64-column block of a key or value tile: 8 KB
 constexpr int kWaStage = 32 * 64;                         // per softmax warp: 32 rows x 32 bf16 of output
@@ -70,6 +71,8 @@ __device__ __forceinline__ WaItem wa_item(const WindowAttnTcParams& p, long long
   it.old -= j_lo;      // from here on: context index of row r relative to the item's first key = old + r
   return it;
 }
+// Rows of the item's last key tile that are the portion's own; behind them come the next portion's, or nobody's.
+__device__ __forceinline__ int wa_own(const WaItem& it) { return it.old + it.len - (it.n_kt - 1) * kWaKeys; }
 
 template <int DB, int RB, int VB>
 __global__ void __launch_bounds__(kWaThreads, 1)
@@ -81,7 +84,7 @@ window_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_c
   constexpr uint32_t kColO = kWaTiles * 2 * kWaKeys;
   static_assert(kColO + kWaTiles * VB * 64 <= kWaTmem, "TMEM columns");
   extern __shared__ unsigned char smem_dyn[];
-  __shared__ uint64_t s_q_full, s_q_empty, s_k_full[2], s_k_empty[2], s_v_full[2], s_v_empty[2], s_drain;
+  __shared__ uint64_t s_q_full, s_q_empty, s_k_full[2], s_k_empty[2], s_v_full[2], s_v_empty[2], s_dirty[2], s_drain;
   __shared__ uint64_t s_s_full[kWaTiles][2], s_p_full[kWaTiles][2], s_o_full[kWaTiles][2];
   __shared__ uint32_t s_tmem_base;
   __shared__ int s_abort;
@@ -97,7 +100,7 @@ window_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_c
     mbar_init(&s_q_full, 1); mbar_init(&s_q_empty, 1); mbar_init(&s_drain, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_k_full[i], 1); mbar_init(&s_k_empty[i], 1);
-      mbar_init(&s_v_full[i], 1); mbar_init(&s_v_empty[i], 1);
+      mbar_init(&s_v_full[i], 1); mbar_init(&s_v_empty[i], 1); mbar_init(&s_dirty[i], 1);
       for (int q = 0; q < kWaTiles; ++q) {
         mbar_init(&s_s_full[q][i], 1);
         mbar_init(&s_p_full[q][i], 4);
@@ -144,10 +147,11 @@ window_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_c
 #pragma unroll
           for (int c = 0; c < RB; ++c) tma_load_2d(ks + (DB + c) * kWaKBlk, &tmap_r, 64 * c, y, &s_k_full[st]);
           if (!(ok = mbar_wait(&s_v_empty[st], ph ^ 1u, abort_flag, p.status, 1))) break;
-          mbar_expect_tx(&s_v_full[st], VB * kWaKBlk);
+          uint64_t* v_full = t + 1 < it.n_kt || wa_own(it) >= kWaKeys ? &s_v_full[st] : &s_dirty[st];
+          mbar_expect_tx(v_full, VB * kWaKBlk);
 #pragma unroll
           for (int c = 0; c < VB; ++c)
-            tma_load_2d(ks + (QB + c) * kWaKBlk, &tmap_v, it.h / p.group * p.v_head + 64 * c, y, &s_v_full[st]);
+            tma_load_2d(ks + (QB + c) * kWaKBlk, &tmap_v, it.h / p.group * p.v_head + 64 * c, y, v_full);
         }
         ++n_it;
       }
@@ -155,6 +159,28 @@ window_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_c
         const unsigned long long w0 = global_ns();
         while (global_ns() - w0 < 1000000ull) {}
       }
+    }
+  } else if (warp == 4 * kWaTiles + 2) {
+    // Weights of keys that are not the portion's own are 0, which would still take an infinity or a NaN from their values into the product.
+    // A tile with such keys comes by the barrier of this warp, which clears their values and hands it on: the others see nothing of it.
+    // (By the issuing thread, whose instructions bound the kernel, it cost 1.5 to 3 %: 438 -> 446 us for portions of 4 x 2048 tokens, 32 heads of 128, window 2048.)
+    uint32_t n_t = 0, n_d[2] = {};
+    for (long long w = blockIdx.x; w < p.n_items; w += gridDim.x) {
+      const WaItem it = wa_item(p, w);
+      if (!it.valid) continue;
+      n_t += (uint32_t)it.n_kt;
+      const int own = wa_own(it);
+      if (own >= kWaKeys) continue;
+      const uint32_t st = (n_t - 1u) & 1u;
+      // Its wait lasts from one portion's end to the next: the limit is that of many of the others' waits.
+      if (!__all_sync(0xffffffffu, mbar_wait(&s_dirty[st], n_d[st]++ & 1u, abort_flag, p.status, 8, 30 * kWaitLimitNs))) break;
+      uint4* rows = reinterpret_cast<uint4*>(kv_smem + st * kStage + QB * kWaKBlk);
+      for (int i = own * 8 + lane; i < kWaKeys * 8; i += 32)
+#pragma unroll
+        for (int c = 0; c < VB; ++c) rows[c * (kWaKBlk / 16) + i] = make_uint4(0u, 0u, 0u, 0u);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s_v_full[st]);
     }
   } else if (warp == 4 * kWaTiles + 1) {
     if (lane == 0) {
