@@ -325,7 +325,9 @@ int msa_lm_rows_gemm(const msa_lm_rows_gemm_args* args, void* stream);
 /* ---- beam search ----------------------------------------------------------------------------------------------------
  * The k best continuations of every question's beams.  Row q * beams + b of logits [batch * beams, vocab] (stride elements
  * apart) belongs to beam b, whose score is scores[q, b]; continuation (b, t) has the score scores[q, b] + x_t - log sum exp x, and
- * score / beam / token [batch, k] receive the best in descending 64-bit order; equals: the lower beam, the larger logit, the lower token.  Logits of
+ * score / beam / token [batch, k] receive the best in descending order; equals: the lower beam, the larger logit, the lower token.  Scores are added
+ * and compared in 64 bits, but a row's sum is good to 5.5e-7 only (1.2e-6 for logits beyond 1e6), in bits that depend on batch * beams: within a beam
+ * the order is that of the logits, and continuations of two beams that are closer than twice that may come in either order.  Logits of
  * -inf are no continuations; neither are those of a beam whose score is not finite or whose row holds a NaN or +inf.  Places left over:
  * (-inf, -1, -1).  live_* [batch, beams] (all or none): the first `beams` of the k whose token is not among stop [n_stop].
  * 1 to 32 beams, k up to 64; workspace: msa_lm_beam_topk_workspace bytes, 8-byte aligned. */

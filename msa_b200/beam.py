@@ -62,7 +62,7 @@ def choose(x: torch.Tensor, scores: torch.Tensor, k: int, stop: Sequence[int]):
     """``beam_topk`` of the ``k`` best, of which ``beams`` go on whatever the others are: stop tokens take at most ``len(stop)`` places a
     beam.  Where that is more than ``beam_topk`` gives, the best are chosen by themselves, and for the beams that go on a row's stop
     tokens are one of their joint probability: log softmax stays what it was (but for the rounding of that one logit), and one place
-    a beam is enough."""
+    a beam is enough; the first three tables then hold ``beams`` places.  ``stop`` is a list on the host."""
     beams, vocab = scores.shape[1], x.shape[1]
     ids = lambda tokens: torch.tensor(tokens, dtype=torch.int32, device=x.device)
     if k >= min(beams * (1 + len(stop)), beams * vocab):

@@ -2,7 +2,9 @@
 //
 // Choice.  A candidate (beam b, token t) has the score  s_b + (x_bt - lse_b),  lse_b = log sum_t exp x_bt.  Within a row the order is
 // that of the logits, so one pass over a row yields its sum and the largest logit of every 512, and a question's k best lie in the k chunks
-// whose largest are the best; the second kernel ranks those, reads them again and ranks what lies in them, in 64 bits.  Bound by the one read
+// whose largest are the best; the second kernel ranks those, reads them again and ranks what lies in them: scores are added and compared in
+// 64 bits, a row's sum (terms of 2^-22, added by sixteen in 32 bits, from there on in 64) is good to 5.5e-7 of itself.  Its last bits depend on the
+// number of parts that the rows are cut into, and so on how many rows there are.  Bound by the one read
 // of the logits (48 x 4 rows of 151,936 fp32: 23 us at 5.1 TB/s, then 8), for few rows by the second kernel's chain of barriers (7 us).
 //
 // Reordering.  New beam j continues beam parent[j].  Its first child keeps a beam's slot, the others take slots that nobody
@@ -96,7 +98,8 @@ beam_rows_kernel(const T* __restrict__ logits, long long stride, const float* __
       top = m; base = new_base; big_n = new_n; floor_x = m - 80.f;
     }
     if (top == -INFINITY) return;
-    // e^x / 2^big_n: the exponent's whole part by integer arithmetic, the fraction (exact to 2^-25) by ex2; two at a time.
+    // e^x / 2^big_n by Cody and Waite's reduction (Software Manual for the Elementary Functions, 1980): x log2 e = n + f with log2 e in two
+    // pieces, n into the exponent by integer arithmetic, 2^f (f exact to 2^-26) by ex2; two at a time.
     if (base == 0.f) {
       const float magic = 12582912.f - big_n;
       const unsigned long long log2e = f32x2(1.44269504f, 1.44269504f), rest = f32x2(1.92596299e-8f, 1.92596299e-8f), magic2 = f32x2(magic, magic),

@@ -14,7 +14,10 @@
 // While one tile's softmax runs, the tensor pipe works for the other.  128 keys because an issued product takes some 70 cycles
 // whatever its columns: with 64 the issuing thread was the bound (3460 cycles for 64 keys of both tiles, 2200 of them issuing).  That
 // thread is kept to one wait for copies, two for P and three commits per 128 keys: each costs it 90 to 140 cycles (4130 cycles an
-// iteration with six of each).  Two issuing threads are slower (368 us where one takes 298).
+// iteration with six of each).  Two issuing threads are slower (368 us where one took 298).
+//
+// Figures here are launches back to back of 4 portions of 2048 tokens, 32 heads over 8 of 128, window 2048, first and second of each pair on the same
+// card, some before later steps and on other cards; as it stands the kernel takes 250 us so.
 //
 // Keys come as slots: the context's first rows up to a multiple of 8, then its rows from `base` on, the first that the item's window
 // reaches (or where those rows end).  A tile in which the two meet is fetched by two copies, so that few first tokens cost no tile.
@@ -99,7 +102,7 @@ __device__ __forceinline__ bool elect_one() {
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(r));
   return r != 0;
 }
-// A store that leaves no line in the L1, which shared memory holds nearly all of: 5 us of 262 for portions of 4 x 2048 tokens.
+// A store that leaves no line in the L1, which shared memory holds nearly all of: 5 us of 262.
 __device__ __forceinline__ void store_once(void* p, uint4 v) {
   asm volatile("st.global.L1::no_allocate.v4.b32 [%0], {%1, %2, %3, %4};" ::"l"(p), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
@@ -248,7 +251,7 @@ first_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     }
   } else if (warp == 4 * kFtTiles + 1) {
     // The whole warp walks along, and one thread (always the same) issues: with the others left behind at a branch around all of this, each
-    // product's descriptors cost more than the product (261 us where this takes 256).
+    // product's descriptors cost more than the product (261 us against 256).
     const uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kFtKeys >> 3) << 17) | ((uint32_t)(kFtRows >> 4) << 24);
     const uint32_t idesc_pv = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(VB * 64 >> 3) << 17) |
                               ((uint32_t)(kFtRows >> 4) << 24);

@@ -166,8 +166,10 @@ def beam_topk(logits: torch.Tensor, scores: torch.Tensor, k: int, stop: Optional
     """The ``k`` best continuations of every question's beams: ``(score fp32, beam, token)``, each ``[batch, k]`` in descending order.
 
     ``scores`` fp32 ``[batch, beams]``; row ``q * beams + b`` of ``logits`` (fp32 or bf16 ``[batch * beams, vocab]``, rows with a
-    contiguous last axis) belongs to beam b of question q.  Continuation (b, t) has the score ``scores[q, b] + log_softmax(row)[t]``, ordered
-    in 64 bits; equals go to the lower beam, then to the larger logit, then to the lower token.  Logits of -inf are no continuations, nor is anything of a beam whose score is not
+    contiguous last axis) belongs to beam b of question q.  Continuation (b, t) has the score ``scores[q, b] + log_softmax(row)[t]``; equals
+    go to the lower beam, then to the larger logit, then to the lower token.  Scores are added and compared in 64 bits, but a row's sum is good
+    to 5.5e-7 only (1.2e-6 for logits beyond 1e6), in bits that depend on the number of rows: within a beam the order is that of the logits, and
+    continuations of two beams closer than twice that may come in either order.  Logits of -inf are no continuations, nor is anything of a beam whose score is not
     finite or whose row holds a NaN or +inf; places left over hold ``(-inf, -1, -1)``.
 
     With ``stop`` (int32 token ids, may be empty) three more, ``[batch, beams]``: the first ``beams`` of the k whose token is not
@@ -349,9 +351,11 @@ GROUP_CLUSTER = 8            # splits of a cluster, at most
 
 
 def splits_join(splits: int, ring_rows: int) -> bool:
-    """Whether a cluster of up to 8 splits, which joins its results in the same launch, beats more of them with a kernel that merges.  16 heads
-    over 4 of 128, one sequence: 12.3 us against 14.3 over 1028 rows, 16.4 against 20.5 over 4100, 22.5 both over 8196 and 32.8 against 24.6 over
-    16,388; 16 sequences, 4 splits in either form: 18.4 against 20.5 over 1028 and 114.7 against 116.7 over 16,388."""
+    """Whether a cluster of up to 8 splits, which joins its results in the same launch, beats more of them with a kernel that merges.  Device times
+    from a graph, one sequence, 16 heads over 4 of 128: 6.5 us against 7.3 over 1028 rows, 10.9 against 12.3 over 4100, 13.7 against 12.8 over
+    6148 and 27.7 against 16.0 over 16,388; 32 over 8 of 128: 7.4 and 8.6, 11.6 and 11.7, 13.9 and 12.3, 27.9 and 17.5; 8 over 1 alike.  (32 over 4 of 64
+    would change at some 10,000 rows: 9.3 and 11.5 over 6148, 10.8 and 11.9 over 8196, 17.0 and 13.2 over 16,388.)  16 sequences, 4 splits in either form:
+    10.7 against 11.5 over 1028 and 93.3 against 93.7 over 16,388.  Calls in a row, with the host's part: 8.2 against 12.3 over 1028."""
     return splits <= GROUP_CLUSTER or ring_rows <= 4608
 
 
