@@ -184,6 +184,8 @@ class SequenceStateCache(SparseCache):
             parts = []
 
             def add(t: torch.Tensor, kind: int, unit: int, rows: int = 0, first: int = 0):
+                if t.shape[0] < self.n_slots or t.device != self.last_token.device or not t[:1].is_contiguous():
+                    raise A.MsaError(f"reorder: {tuple(t.shape)} is not the state of {self.n_slots} slots on {self.last_token.device}, each contiguous")
                 slot = t.stride(0) * t.element_size()
                 if unit and t.shape[0]:
                     align = next(a for a in (16, 4, 2) if not (t.data_ptr() % a or slot % a or unit % a))

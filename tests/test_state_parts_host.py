@@ -37,3 +37,16 @@ def test_the_last_tokens_and_all_rings_at_once():
 def test_the_table_is_made_once():
     c = cache()
     assert c._state_parts() is c._state_parts()
+
+
+@pytest.mark.parametrize("bad", ["few slots", "order", "device"])
+def test_a_tensor_that_is_no_state_is_refused(bad):
+    from msa_b200 import _cabi_lm as A
+    c = cache()
+    bases(c)
+    t = c.ring[0]
+    c.ring[0] = {"few slots": t[:1], "order": t.transpose(1, 2).contiguous().transpose(1, 2), "device": t.to("meta")}[bad]
+    with pytest.raises(A.MsaError):
+        c._state_parts()
+    c.ring[0] = t.clone()
+    assert c.ring[0].data_ptr() in bases(c)
